@@ -240,7 +240,7 @@ def _own_experts(s):
     import rocm_sgemm_b200 as sg
     c, a, b = s["case"], s["a"], s["b"]
     sg.gemm_mx4_grouped(sg.mx4_format[c["fmt"]], sg.m_type[c["type"]], s["c"], a[0], a[1], b[0], b[1], s["c"].shape[0], c["n"], c["k"],
-                        c["experts"], s["offsets"], s["counts"], global_a=a[2], global_b=b[2])
+                        c["experts"], s["offsets"], s["counts"], used_rows=c["tokens"] * c["top_k"], global_a=a[2], global_b=b[2])
     return s["c"]
 
 
