@@ -283,6 +283,108 @@ int b200_sgemm_release_stream(void* cuda_stream);
 /* Frees the internal split-K arenas of every device (optional; they are also freed at unload). */
 int b200_sgemm_shutdown(void);
 
+/* ---- 4-bit products -------------------------------------------------------------------------------------------
+ * Matrices in microscaled 4-bit floating point (e2m1 codes, one scale per block of neighbours along the summed
+ * dimension K), their product on the tensor cores, the same product for rows sorted into groups that each have a
+ * right-hand matrix of their own (the experts of a mixture), and the sorting of rows that it needs.  Not part of the
+ * reference's surface.  Pointers are device pointers; every entry is asynchronous on `cuda_stream`, allocates nothing,
+ * keeps nothing between calls and can be captured into a graph and replayed on any stream; calls on different streams share
+ * nothing.  Zero extents are B200_SGEMM_INVALID_ARGUMENT, extents above 2^30 B200_SGEMM_UNSUPPORTED_SIZE. */
+
+/* element types of sources and results */
+#define B200_SGEMM_F32 0
+#define B200_SGEMM_F16 1
+#define B200_SGEMM_BF16 2
+
+/* formats: NVFP4 has a block of 16 with an e4m3 scale, times one FP32 scale for the whole matrix; MXFP4 a block of 32 with a
+ * power of two (e8m0) and nothing else. */
+#define B200_SGEMM_NVFP4 0
+#define B200_SGEMM_MXFP4 1
+
+/* Bytes of the two arrays of a quantised rows x K matrix (0: bad format or extent).
+ * codes: rows of ceil(K / 32) * 16 bytes, byte b holds k = 2b in its lower and k = 2b + 1 in its upper half.
+ * scales: one byte per row and block in tiles of 128 rows x 4 blocks (512 bytes: row r, block c at (r % 32) * 16
+ * + (r % 128) / 32 * 4 + c % 4); the tiles of a band of 128 rows follow each other along K, the bands one another.
+ * Codes and scales behind K, in the last 16 bytes of a row and the last tile of a band, have to be zero where another program
+ * writes them; b200_sgemm_mx4_quantize writes them so.  Both arrays start on 16 bytes. */
+size_t b200_sgemm_mx4_code_bytes(int format, size_t rows, size_t K);
+size_t b200_sgemm_mx4_scale_bytes(int format, size_t rows, size_t K);
+
+/* X (rows x K, `type`, row-major with ldx >= K or col-major with ldx >= rows; 0 = packed) to codes and scales.  K is the
+ * dimension that a product sums over, so the left matrix A (M x K) is quantised as it is and the right one (K x N) as its
+ * transpose: N rows, and the other layout.  In exact arithmetic, RN = to nearest, ties to the even code:
+ *   NVFP4  s = RN_e4m3(amax / (6 g)), at most 448;    code = RN_e2m1(x / (s g)), at most 6; g = *global_scale, 1 if NULL
+ *   MXFP4  s = 2^(floor(log2 amax) - 2), in 2^+-127;  code = RN_e2m1(x / s), at most 6; global_scale has to be NULL
+ * with amax the block's largest magnitude.  s = 0 gives zero codes.  A block with an infinity or a NaN has the NaN scale
+ * (0x7F, 0xFF) and zero codes; a g that is not in 2^-90 .. 2^90 gives NaN scales everywhere.  The values that stand
+ * for X are code * s * g.
+ * row_index (NULL: none; row-major X only): row r is X row row_index[r] / index_div, X has source_rows rows; a negative index
+ * or one behind X leaves the codes of row r as they were and its scales zero, and a band of 128 rows without any
+ * valid index is not written at all.  With the row_slot of b200_sgemm_route_sort and index_div = top_k this sorts tokens and
+ * quantises them in one pass.  Without row_index source_rows is 0 and index_div ignored. */
+int b200_sgemm_mx4_quantize(int format, int layout, int type, const void* X, size_t rows, size_t K, size_t ldx,
+                            const int* row_index, size_t source_rows, int index_div, const float* global_scale, void* codes,
+                            void* scales, void* cuda_stream);
+
+/* The values that codes and scales stand for: X (rows x K, row-major, ldx >= K, 0 = packed) = code * s * g, one rounding to
+ * FP32 and one to `type`. */
+int b200_sgemm_mx4_dequantize(int format, int type, const void* codes, const void* scales, size_t rows, size_t K,
+                              const float* global_scale, void* X, size_t ldx, void* cuda_stream);
+
+/* C[m, n] = alpha * global_a * global_b * sum_k A[m, k] B[n, k] from two quantised matrices of the same format, A of M and
+ * B of N rows of K.  C is of `type_c`, row-major (ldc >= N) or col-major (ldc >= M; 0 = packed), overwritten.  Sums are kept
+ * in FP32 and rounded to type_c once.  global_a / global_b: one device float each or NULL (1); NULL for MXFP4.  A few rows on
+ * one side (the tokens of a decode step) are a case of its own: the long matrix streams through at the memory's rate. */
+int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
+                   const void* b_scales, size_t M, size_t N, size_t K, size_t ldc, float alpha, const float* global_a,
+                   const float* global_b, void* cuda_stream);
+
+/* The product for `groups` (<= 1024) groups of rows: for every row m in offsets[e] .. offsets[e] + counts[e] - 1
+ *   C[m, n] = alpha * global_a * global_b[e] * sum_k A[m, k] B_e[n, k]
+ * A: rows x K quantised once; B: `groups` matrices of N x K, codes one after the other and scales one after the other (each
+ * as its own b200_sgemm_mx4_code_bytes / _scale_bytes); global_b: one float per group.  C: rows x N, row-major, ldc >= N;
+ * rows in no group are left as they were.  offsets and counts live on the device, so nothing waits for the host; offsets are
+ * multiples of 128 (b200_sgemm_route_sort with align = 128 makes them so), groups without rows cost nothing.  A group whose
+ * offset or count does not fit is left out and reported by b200_sgemm_mx4_device_status.  used_rows (0: not known): about how
+ * many rows the groups hold in all; it only chooses the tile. */
+int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
+                           const void* b_scales, size_t rows, size_t N, size_t K, size_t ldc, size_t groups, const int* offsets,
+                           const int* counts, size_t used_rows, float alpha, const float* global_a, const float* global_b,
+                           void* cuda_stream);
+
+/* Synchronises the current device, then reads and clears the status word of the two products: 0 = no kernel reported a
+ * problem; bit 0: a bounded wait inside a kernel gave up (its result is invalid), bit 1: a group was left out. */
+int b200_sgemm_mx4_device_status(int* status);
+
+/* Routing: every one of `tokens` tokens has top_k slots, slot t * top_k + j naming an expert (0 .. experts-1; anything else
+ * drops the slot).  A token may name an expert twice.
+ *
+ * b200_sgemm_route_sort sorts the slots by expert, stable in the slot number: expert e's slots take rows offsets[e] ..
+ * offsets[e] + counts[e] - 1 in order; offsets are multiples of `align`, offsets[experts] is the end of the last
+ * expert's rows rounded up.  slot_row[slot] = the slot's row or -1; row_slot[row] = the row's slot or -1, for all `rows` rows.
+ * rows is at least b200_sgemm_route_capacity(tokens, top_k, experts, align), which no routing exceeds.  experts <= 1024. */
+size_t b200_sgemm_route_capacity(size_t tokens, size_t top_k, size_t experts, size_t align);
+int b200_sgemm_route_sort(const int* expert_ids, size_t tokens, size_t top_k, size_t experts, size_t align, int* offsets,
+                          int* counts, int* slot_row, int* row_slot, size_t rows, void* cuda_stream);
+
+/* Xs[slot_row[t * top_k + j]] = X[t]: X tokens x width, Xs rows x width, row-major, ldx / lds >= width (0 = packed), same
+ * type.  Rows that no slot names are left as they were.  A slot_row outside 0 .. rows-1 counts as dropped, here and below. */
+int b200_sgemm_route_dispatch(int type, const void* X, size_t tokens, size_t width, size_t ldx, const int* slot_row, size_t top_k,
+                              void* Xs, size_t rows, size_t lds, void* cuda_stream);
+
+/* out[t] = sum_j weights[t * top_k + j] * Y[slot_row[t * top_k + j]] over the token's kept slots, in ascending j in
+ * FP32, rounded once; zero for a token without any.  weights FP32, NULL: all 1 - which is the gradient of
+ * b200_sgemm_route_dispatch with respect to X. */
+int b200_sgemm_route_combine(int type, const void* Y, size_t rows, size_t width, size_t ldy, const int* slot_row, size_t tokens,
+                             size_t top_k, const float* weights, void* out, size_t ldo, void* cuda_stream);
+
+/* The gradients of b200_sgemm_route_combine: dY[slot_row[s]] = weights[s] * d_out[t] (rows that no slot names are left as they
+ * were) and d_weights[s] = sum over the width of d_out[t] * Y[slot_row[s]] in FP32, 0 for a dropped slot.  weights NULL: all
+ * 1.  dY or d_weights may be NULL (not both): not wanted; Y is needed for d_weights only. */
+int b200_sgemm_route_combine_backward(int type, const void* d_out, size_t ldo, const void* Y, size_t rows, size_t width, size_t ldy,
+                                      const int* slot_row, size_t tokens, size_t top_k, const float* weights, void* dY,
+                                      size_t lddy, float* d_weights, void* cuda_stream);
+
 /* Human-readable text for a status returned by any function above. */
 const char* b200_sgemm_status_string(int status);
 

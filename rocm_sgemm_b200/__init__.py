@@ -31,6 +31,20 @@ class m_layout(enum.IntEnum):
 
 ROW, COL = m_layout.row_major, m_layout.col_major
 
+
+class m_type(enum.IntEnum):
+    """Element type of the sources and results of the 4-bit and routing entries."""
+    f32 = 0
+    f16 = 1
+    bf16 = 2
+
+
+class mx4_format(enum.IntEnum):
+    """Microscaled 4-bit formats: e2m1 codes with an e4m3 scale per 16 (nvfp4) or a power of two per 32 (mxfp4)."""
+    nvfp4 = 0
+    mxfp4 = 1
+
+
 OK = 0
 INVALID_ARGUMENT = -1
 NO_KERNEL = -2
@@ -91,7 +105,10 @@ EXPORTS = ("b200_sgemm", "b200_sgemm_ex", "b200_sgemm_workspace_bytes", "b200_sg
            "b200_sgemm_status_string", "b200_sgemm_3xtf32", "b200_sgemm_3xtf32_device_status",
            "b200_sgemm_3xtf32_shutdown", "b200_sgemm_strided_batched", "b200_sgemm_blas",
            "b200_sgemm_blas_shutdown", "b200_sgemm_multi", "b200_sgemm_stream_plan",
-           "b200_sgemm_selftest_bounded_wait", "b200_sgemm_trial")
+           "b200_sgemm_selftest_bounded_wait", "b200_sgemm_trial", "b200_sgemm_mx4_code_bytes", "b200_sgemm_mx4_scale_bytes",
+           "b200_sgemm_mx4_quantize", "b200_sgemm_mx4_dequantize", "b200_sgemm_mx4", "b200_sgemm_mx4_grouped",
+           "b200_sgemm_mx4_device_status", "b200_sgemm_route_capacity", "b200_sgemm_route_sort", "b200_sgemm_route_dispatch",
+           "b200_sgemm_route_combine", "b200_sgemm_route_combine_backward")
 
 
 def lib() -> ctypes.CDLL:
@@ -131,6 +148,22 @@ def lib() -> ctypes.CDLL:
     l.b200_sgemm_stream_plan.argtypes = [i, i, i, _sz, _sz, _sz, i, i, i, ip, ip, ip, i]
     l.b200_sgemm_selftest_bounded_wait.argtypes = [_vp, _vp, _vp, _vp]
     l.b200_sgemm_trial.argtypes = [i, i, i, _vp, _vp, _vp, _sz, _sz, _sz, i, i, i, _vp]
+    for name, args, result in (
+            ("b200_sgemm_mx4_code_bytes", [i, _sz, _sz], _sz),
+            ("b200_sgemm_mx4_scale_bytes", [i, _sz, _sz], _sz),
+            ("b200_sgemm_mx4_quantize", [i, i, i, _vp, _sz, _sz, _sz, _vp, _sz, i, _vp, _vp, _vp, _vp], i),
+            ("b200_sgemm_mx4_dequantize", [i, i, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp], i),
+            ("b200_sgemm_mx4", [i, i, i] + [_vp] * 5 + [_sz] * 4 + [ctypes.c_float, _vp, _vp, _vp], i),
+            ("b200_sgemm_mx4_grouped", [i, i] + [_vp] * 5 + [_sz] * 5 + [_vp, _vp, _sz, ctypes.c_float, _vp, _vp, _vp], i),
+            ("b200_sgemm_mx4_device_status", [ip], i),
+            ("b200_sgemm_route_capacity", [_sz] * 4, _sz),
+            ("b200_sgemm_route_sort", [_vp] + [_sz] * 4 + [_vp] * 4 + [_sz, _vp], i),
+            ("b200_sgemm_route_dispatch", [i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp], i),
+            ("b200_sgemm_route_combine", [i, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp], i),
+            ("b200_sgemm_route_combine_backward",
+             [i, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _vp], i)):
+        getattr(l, name).argtypes = args
+        getattr(l, name).restype = result
     l.b200_sgemm_status_string.argtypes = [i]
     l.b200_sgemm_status_string.restype = ctypes.c_char_p
     _lib = l
@@ -364,6 +397,82 @@ def device_status() -> int:
     st = ctypes.c_int(0)
     _check(lib().b200_sgemm_device_status(ctypes.byref(st)))
     return st.value
+
+
+def mx4_sizes(fmt, rows: int, K: int) -> tuple:
+    """(bytes of the codes, bytes of the scales) of a quantised rows x K matrix."""
+    return (int(lib().b200_sgemm_mx4_code_bytes(fmt, rows, K)), int(lib().b200_sgemm_mx4_scale_bytes(fmt, rows, K)))
+
+
+def mx4_quantize(fmt, layout, dtype, X, rows: int, K: int, codes, scales, ldx: int = 0, row_index=None, source_rows: int = 0,
+                 index_div: int = 1, global_scale=None, stream=None) -> None:
+    """X (rows x K, K the summed dimension; row- or col-major) to 4-bit codes and block scales (b200_sgemm_mx4_quantize).
+    row_index: row r is X row row_index[r] // index_div of source_rows."""
+    _check(lib().b200_sgemm_mx4_quantize(fmt, layout, dtype, _ptr(X), rows, K, ldx, _ptr(row_index), source_rows, index_div,
+                                         _ptr(global_scale), _ptr(codes), _ptr(scales), _stream(stream)))
+
+
+def mx4_dequantize(fmt, dtype, codes, scales, rows: int, K: int, X, ldx: int = 0, global_scale=None, stream=None) -> None:
+    """The values that codes and scales stand for, as a row-major rows x K matrix (b200_sgemm_mx4_dequantize)."""
+    _check(lib().b200_sgemm_mx4_dequantize(fmt, dtype, _ptr(codes), _ptr(scales), rows, K, _ptr(global_scale), _ptr(X), ldx,
+                                           _stream(stream)))
+
+
+def gemm_mx4(fmt, layout_c, dtype_c, C, A_codes, A_scales, B_codes, B_scales, M: int, N: int, K: int, ldc: int = 0,
+             alpha: float = 1.0, global_a=None, global_b=None, stream=None) -> None:
+    """C = alpha * global_a * global_b * A @ B from a quantised A (M rows of K) and B (N rows of K) (b200_sgemm_mx4)."""
+    _check(lib().b200_sgemm_mx4(fmt, layout_c, dtype_c, _ptr(C), _ptr(A_codes), _ptr(A_scales), _ptr(B_codes), _ptr(B_scales),
+                                M, N, K, ldc, alpha, _ptr(global_a), _ptr(global_b), _stream(stream)))
+
+
+def gemm_mx4_grouped(fmt, dtype_c, C, A_codes, A_scales, B_codes, B_scales, rows: int, N: int, K: int, groups: int, offsets,
+                     counts, ldc: int = 0, used_rows: int = 0, alpha: float = 1.0, global_a=None, global_b=None,
+                     stream=None) -> None:
+    """The product for rows offsets[e] .. + counts[e] of A with matrix e of B, for every group e (b200_sgemm_mx4_grouped)."""
+    _check(lib().b200_sgemm_mx4_grouped(fmt, dtype_c, _ptr(C), _ptr(A_codes), _ptr(A_scales), _ptr(B_codes), _ptr(B_scales), rows,
+                                        N, K, ldc, groups, _ptr(offsets), _ptr(counts), used_rows, alpha, _ptr(global_a),
+                                        _ptr(global_b), _stream(stream)))
+
+
+def mx4_device_status() -> int:
+    """Synchronises the current device and returns (then clears) the 4-bit products' status word; 0 = healthy."""
+    st = ctypes.c_int(0)
+    _check(lib().b200_sgemm_mx4_device_status(ctypes.byref(st)))
+    return st.value
+
+
+def route_capacity(tokens: int, top_k: int, experts: int, align: int) -> int:
+    """Rows that sorting tokens * top_k slots by expert can take at most."""
+    return int(lib().b200_sgemm_route_capacity(tokens, top_k, experts, align))
+
+
+def route_sort(expert_ids, tokens: int, top_k: int, experts: int, align: int, offsets, counts, slot_row, row_slot, rows: int,
+               stream=None) -> None:
+    """Sorts slots by expert: int32 offsets[experts + 1], counts[experts], slot_row[tokens * top_k], row_slot[rows]
+    (b200_sgemm_route_sort)."""
+    _check(lib().b200_sgemm_route_sort(_ptr(expert_ids), tokens, top_k, experts, align, _ptr(offsets), _ptr(counts),
+                                       _ptr(slot_row), _ptr(row_slot), rows, _stream(stream)))
+
+
+def route_dispatch(dtype, X, tokens: int, width: int, slot_row, top_k: int, Xs, rows: int, ldx: int = 0, lds: int = 0,
+                   stream=None) -> None:
+    """Xs[slot_row[t, j]] = X[t] (b200_sgemm_route_dispatch)."""
+    _check(lib().b200_sgemm_route_dispatch(dtype, _ptr(X), tokens, width, ldx, _ptr(slot_row), top_k, _ptr(Xs), rows, lds,
+                                           _stream(stream)))
+
+
+def route_combine(dtype, Y, rows: int, width: int, slot_row, tokens: int, top_k: int, out, weights=None, ldy: int = 0,
+                  ldo: int = 0, stream=None) -> None:
+    """out[t] = sum over j of weights[t, j] * Y[slot_row[t, j]]; without weights the gradient of route_dispatch."""
+    _check(lib().b200_sgemm_route_combine(dtype, _ptr(Y), rows, width, ldy, _ptr(slot_row), tokens, top_k, _ptr(weights),
+                                          _ptr(out), ldo, _stream(stream)))
+
+
+def route_combine_backward(dtype, d_out, Y, rows: int, width: int, slot_row, tokens: int, top_k: int, weights, dY, d_weights,
+                           ldo: int = 0, ldy: int = 0, lddy: int = 0, stream=None) -> None:
+    """Gradients of route_combine: dY[slot_row[t, j]] = weights[t, j] * d_out[t], d_weights[t, j] = <d_out[t], Y[...]>."""
+    _check(lib().b200_sgemm_route_combine_backward(dtype, _ptr(d_out), ldo, _ptr(Y), rows, width, ldy, _ptr(slot_row), tokens,
+                                                   top_k, _ptr(weights), _ptr(dY), lddy, _ptr(d_weights), _stream(stream)))
 
 
 def release_stream(stream=None) -> None:

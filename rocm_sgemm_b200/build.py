@@ -108,7 +108,12 @@ def build_library(config: Path | None = None, jobs: int | None = None, verbose=F
     work.append((CSRC / "sgemm_api.cu", api_deps))
     work.append((CSRC / "sgemm_static_scratch.cu", [REPO / "include" / "b200_sgemm.h"]))
     work.append((CSRC / "sgemm_host.cu", [REPO / "include" / "b200_sgemm.h"]))
-    work.append((CSRC / "sgemm_tf32x3.cu", kernel_hdr + [CSRC / "transpose.hpp", REPO / "include" / "b200_sgemm.h"]))
+    work.append((CSRC / "sgemm_tf32x3.cu",
+                 kernel_hdr + [CSRC / "tcgen05.cuh", CSRC / "transpose.hpp", REPO / "include" / "b200_sgemm.h"]))
+    mx4_deps = [CSRC / "mx4_common.cuh", REPO / "include" / "b200_sgemm.h"]
+    work.append((CSRC / "mx4_quantize.cu", mx4_deps))
+    work.append((CSRC / "mx4_gemm.cu", mx4_deps + kernel_hdr + [CSRC / "tcgen05.cuh"]))
+    work.append((CSRC / "route.cu", mx4_deps))
     work.append((CSRC / "sgemm_blas.cu", [REPO / "include" / "b200_sgemm.h"]))
     work.append((CSRC / "sgemm_selftest.cu", kernel_hdr + [REPO / "include" / "b200_sgemm.h"]))
     objs = []

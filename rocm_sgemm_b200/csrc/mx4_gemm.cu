@@ -1,0 +1,755 @@
+// b200_sgemm_mx4 and b200_sgemm_mx4_grouped: products of matrices in microscaled 4-bit floating point on the tensor
+// cores (tcgen05, block-scaled e2m1 operands, FP32 accumulators in tensor memory).
+//
+//   C[m, n] = alpha * global_a * global_b[e] * sum_k A[m, k] B[n, k]
+//
+// Both operands are K-contiguous, so either can take either side of a tile.  The kernel knows a LANE operand P (128 rows
+// of it on the 128 lanes of tensor memory) and a COLUMN operand Q (BN rows of it as columns):
+//   lanes    the dimension along which C is contiguous, so that a warp stores 32 neighbours of C at once; for few tokens
+//            that is the weights, and the tokens cost BN = 32 columns instead of a tile of 128 rows
+//   columns  the other one; the rows of the groups in the grouped product
+//
+// One persistent CTA per SM, 10 warps:
+//   warps 0-7  accumulate and store.  The tensor core adds into its FP32 accumulator with truncation, so for an FP32
+//              result the accumulator is emptied into registers every CHUNK_F32 K blocks and the parts are added there,
+//              rounded to nearest; results of 16 bits keep one accumulator for the whole of K (the bias, measured below
+//              1e-5 of the result at K = 16384, is a hundredth of their rounding).
+//   warp 8     one thread fetches the stages: the two operands' codes by TMA (256 k = 128-byte rows, 128-byte swizzle; zero
+//              beyond the matrix), the scale tiles as they lie by bulk copies
+//   warp 9     one thread copies the stage's scale tiles into tensor memory (tcgen05.cp, replicated to the four lane
+//              quarters) and issues the products, 64 k each.  Scales go to a tensor-memory slot of the stage's own, which is
+//              free as soon as the stage is.
+// Few tiles: a cluster of 2, 4 or 8 CTAs shares a tile, each with a range of K of its own; the parts meet through
+// distributed shared memory and are added in ascending order of K, so the result does not depend on timing and no
+// workspace is needed (a captured graph can be replayed on any stream).
+// Every wait is bounded, as in the other kernels.
+#include "mx4_common.cuh"
+#include "sgemm_ws_kernel.cuh"
+#include "tcgen05.cuh"
+
+#include <cuda.h>
+
+#include <atomic>
+
+namespace
+{
+using namespace sgemm_b200;
+
+constexpr int G_BP        = 128; // lane tile
+constexpr int G_KBLOCK    = 256; // k of one stage: a 128-byte row of codes
+constexpr int G_ROW_BYTES = G_KBLOCK / 2;
+constexpr int G_KSTEP     = 64; // k of one instruction
+constexpr int G_EPILOGUE  = 256;
+constexpr int G_TMA_WARP  = 8;
+constexpr int G_MMA_WARP  = 9;
+constexpr int G_THREADS   = 320;
+constexpr int G_TMEM_COLS = 512;
+constexpr int G_SCALE_COL = 256; // tensor-memory columns 0..255: two accumulators, then 32 of scales per stage
+constexpr int G_MAX_GROUPS = 1024;
+constexpr int CHUNK_F32   = 2;  // K blocks (512 k, 8 products) added inside the tensor core for an FP32 result
+constexpr int G_SCALE_BYTES = 4 * MX4_TILE_BYTES; // of one operand in a stage
+
+constexpr int G_ERR_WAIT  = 1; // status bits: a wait gave up (bits 8.. say which);
+constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the matrix, the group was left out
+
+__device__ int g_mx4_status;
+
+template<int BN>
+struct GLayout
+{
+    static constexpr int    P_BYTES     = G_BP * G_ROW_BYTES;
+    static constexpr int    Q_BYTES     = BN * G_ROW_BYTES;
+    static constexpr int    STAGE_BYTES = P_BYTES + Q_BYTES + 2 * G_SCALE_BYTES;
+    static constexpr int    STAGES      = BN == 128 ? 6 : (BN == 64 ? 7 : 8);
+    static constexpr int    BARRIERS    = 2 * STAGES + 5;
+    static constexpr size_t SMEM_BYTES  = size_t(STAGES) * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers, misc*/;
+    static_assert(8 * BARRIERS + 16 <= 256, "barrier area");
+    static_assert(STAGE_BYTES % 1024 == 0, "swizzled tiles start on 1024 bytes");
+    static_assert(STAGES * 32 + G_SCALE_COL <= G_TMEM_COLS && 2 * BN <= G_SCALE_COL, "tensor memory");
+    static_assert(BN * G_BP * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile lie in the ring");
+};
+
+struct GArgs
+{
+    void*          c;
+    long long      sp, sq; // element strides of C along lanes and columns; one of them is 1
+    const uint8_t* scales_p;
+    const uint8_t* scales_q;
+    const int*     offsets; // grouped: first row (of Q and C) of each group, and rows
+    const int*     counts;
+    const float*   global_p;
+    const float*   global_q;
+    float          alpha;
+    int            np;      // lane extent (of one group's operand)
+    int            nq;      // column extent: rows of Q
+    int            K, kblocks, chunk;
+    int            k_tiles; // scale tiles along k
+    int            tiles_p, bands_p;
+    int            groups;  // 0: one product
+    int            split;   // CTAs of a cluster that share a tile
+    int            type;
+};
+
+// ---- instructions ----------------------------------------------------------------------------------------
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+// a scale tile (32 rows of 16 bytes) to four columns of all four lane quarters
+__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template<int FMT>
+__device__ __forceinline__ void tc_mma_mx4(uint32_t d, uint64_t p_desc, uint64_t q_desc, uint32_t idesc, uint32_t sf_p, uint32_t sf_q,
+                                           uint32_t accumulate)
+{
+    if(FMT == B200_SGEMM_NVFP4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(sf_p), "r"(sf_q), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(sf_p), "r"(sf_q), "r"(accumulate)
+                     : "memory");
+}
+// codes: rows of 128 bytes with the 128-byte swizzle, 1024 bytes between groups of eight rows
+__device__ __forceinline__ uint64_t codes_desc(uint32_t addr)
+{
+    return uint64_t((addr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46)
+           | (uint64_t(2) << 61);
+}
+// scale tile: rows of 16 bytes, no swizzle, 128 bytes between groups of eight rows
+__device__ __forceinline__ uint64_t scales_desc(uint32_t addr)
+{
+    return uint64_t((addr & 0x3FFFFu) >> 4) | (uint64_t(128 >> 4) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+// block-scaled product: e2m1 operands (1), both K-major, N >> 3, scale type (0 e4m3, 1 e8m0), M >> 4; which bytes of the
+// 32-bit scale words an instruction takes is added by the issuer (bits 4-5 for Q, 29-30 for P)
+template<int FMT, int BN>
+__device__ __forceinline__ constexpr uint32_t mx4_idesc()
+{
+    return (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (FMT == B200_SGEMM_MXFP4 ? 1u << 23 : 0u)
+           | (uint32_t(G_BP >> 4) << 24);
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank)
+{
+    uint32_t at;
+    float    v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+// what is in flight when a CTA gives up has to land before it leaves; bounded, without looking at the abort flag
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity)
+{
+    const uint64_t t0 = global_timer_ns();
+    while(!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < 100ull * 1000 * 1000) {}
+}
+
+// ---- tiles -------------------------------------------------------------------------------------------------
+struct Tile
+{
+    int group, p0, q0, q_end; // columns q0 .. min(q0 + BN, q_end)
+};
+// one product: bands of 16 lane tiles, columns advancing inside a band, so that CTAs running together share operands in
+// the L2; groups: all lane tiles of a group's column tile, then the next column tile, so a group's weights stay in the L2
+template<int BN>
+__device__ __forceinline__ Tile tile_at(const GArgs& a, const int* first_tile, int tile)
+{
+    Tile t;
+    if(a.groups == 0)
+    {
+        constexpr int BAND = 16;
+        const int tiles_q = (a.nq + BN - 1) / BN;
+        const int band = tile / (BAND * tiles_q), in = tile - band * BAND * tiles_q;
+        const int wide = min(BAND, a.tiles_p - band * BAND);
+        t.group = 0;
+        t.p0    = (band * BAND + in % wide) * G_BP;
+        t.q0    = in / wide * BN;
+        t.q_end = a.nq;
+        return t;
+    }
+    const int qt = tile / a.tiles_p;
+    int       lo = 0, hi = a.groups; // the group with first_tile[lo] <= qt < first_tile[lo + 1]
+    while(hi - lo > 1)
+    {
+        const int mid = (lo + hi) >> 1;
+        if(first_tile[mid] <= qt)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const int off = a.offsets[lo];
+    t.group = lo;
+    t.p0    = (tile - qt * a.tiles_p) * G_BP;
+    t.q0    = off + (qt - first_tile[lo]) * BN;
+    t.q_end = off + a.counts[lo];
+    return t;
+}
+
+template<class T, int COLS>
+__device__ __forceinline__ void store_columns(const GArgs& a, const float (&acc)[COLS], float factor, int p, int q0, int q_end)
+{
+    if(p >= a.np)
+        return;
+    T* c = static_cast<T*>(a.c) + (long long)p * a.sp + (long long)q0 * a.sq;
+    if(a.sq == 1)
+    {
+        constexpr int N = Vec16<T>::N;
+        const bool vector = ((reinterpret_cast<uintptr_t>(c)) & 15) == 0;
+#pragma unroll
+        for(int j = 0; j < COLS; j += N)
+        {
+            Vec16<T> v;
+#pragma unroll
+            for(int i = 0; i < N; ++i)
+                v.v[i] = from_float<T>(acc[j + i] * factor);
+            if(vector && q0 + j + N <= q_end)
+                *reinterpret_cast<uint4*>(c + j) = v.raw;
+            else
+            {
+#pragma unroll
+                for(int i = 0; i < N; ++i)
+                    if(q0 + j + i < q_end)
+                        c[j + i] = v.v[i];
+            }
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int j = 0; j < COLS; ++j)
+            if(q0 + j < q_end)
+                c[(long long)j * a.sq] = from_float<T>(acc[j] * factor);
+    }
+}
+template<int COLS>
+__device__ __forceinline__ void store_typed(const GArgs& a, const float (&acc)[COLS], float factor, int p, int q0, int q_end)
+{
+    if(a.type == B200_SGEMM_F32)
+        store_columns<float>(a, acc, factor, p, q0, q_end);
+    else if(a.type == B200_SGEMM_F16)
+        store_columns<__half>(a, acc, factor, p, q0, q_end);
+    else
+        store_columns<__nv_bfloat16>(a, acc, factor, p, q0, q_end);
+}
+
+template<int FMT, int BN>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q)
+{
+    using L = GLayout<BN>;
+    constexpr int STAGES      = L::STAGES;
+    constexpr int STAGE_TILES = G_KBLOCK / (4 * mx4_block(FMT)); // scale tiles of a stage, per operand
+    constexpr int COLS        = BN / 2;                          // columns of one epilogue thread
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int first_tile[G_MAX_GROUPS + 1];
+    const uint32_t raw_addr = (uint32_t)__cvta_generic_to_shared(smem_raw);
+    const uint32_t base     = (raw_addr + 1023u) & ~1023u;
+    uint8_t*       ring     = smem_raw + (base - raw_addr);
+    const uint32_t bar_base = base + STAGES * L::STAGE_BYTES;
+    auto full      = [&](int s) { return bar_base + 8u * s; };
+    auto empty     = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    auto acc_full  = [&](int b) { return bar_base + 8u * (2 * STAGES + b); };
+    auto acc_empty = [&](int b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
+    const uint32_t drained = bar_base + 8u * (2 * STAGES + 4);
+    uint8_t*       misc       = ring + STAGES * L::STAGE_BYTES + 8 * L::BARRIERS;
+    uint32_t*      tmem_slot  = reinterpret_cast<uint32_t*>(misc);
+    volatile int*  abort_flag = reinterpret_cast<volatile int*>(misc + 8);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if(threadIdx.x == 0)
+    {
+        for(int s = 0; s < STAGES; ++s)
+        {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for(int b = 0; b < 2; ++b)
+        {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), G_EPILOGUE / 32);
+        }
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if(warp == G_MMA_WARP)
+    {
+        tmem_alloc((uint32_t)__cvta_generic_to_shared(tmem_slot), G_TMEM_COLS);
+        tmem_relinquish();
+    }
+    if(warp == G_TMA_WARP && a.groups) // column tiles before each group
+    {
+        int sum = 0;
+        for(int e0 = 0; e0 < a.groups; e0 += 32)
+        {
+            const int e = e0 + lane;
+            int       n = 0;
+            if(e < a.groups)
+            {
+                const int off = a.offsets[e], count = a.counts[e];
+                if(count > 0 && off >= 0 && off % MX4_BAND == 0 && count <= a.nq && off <= a.nq - count)
+                    n = (count + BN - 1) / BN;
+                else if(count != 0 && blockIdx.x == 0)
+                    atomicOr(&g_mx4_status, G_ERR_GROUP);
+            }
+            int up = n;
+#pragma unroll
+            for(int d = 1; d < 32; d <<= 1)
+            {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, up, d);
+                if(lane >= d)
+                    up += v;
+            }
+            if(e < a.groups)
+                first_tile[e] = sum + up - n;
+            sum += __shfl_sync(0xFFFFFFFFu, up, 31);
+        }
+        if(lane == 0)
+            first_tile[a.groups] = sum;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int split = a.split, rank = split > 1 ? (int)(blockIdx.x % split) : 0;
+    const int first = blockIdx.x / split, stride = gridDim.x / split;
+    const int total = (a.groups ? first_tile[a.groups] : (a.nq + BN - 1) / BN) * a.tiles_p;
+    const int kb0 = (int)((long long)a.kblocks * rank / split), kb1 = (int)((long long)a.kblocks * (rank + 1) / split);
+    // the first wait of the CTA that gives up records where (bits 8..) and raises the abort flag for the others
+    auto fail = [&](int where) {
+        if(atomicExch(const_cast<int*>(abort_flag), 1) == 0)
+            atomicOr(&g_mx4_status, G_ERR_WAIT | (256 << where));
+    };
+
+    if(warp == G_TMA_WARP)
+    {
+        if(lane == 0)
+        {
+            uint32_t it = 0;
+            bool     ok = true;
+            for(int tile = first; tile < total && ok; tile += stride)
+            {
+                const Tile     t   = tile_at<BN>(a, first_tile, tile);
+                const uint8_t* sfp = a.scales_p + (size_t)(t.group * a.bands_p + t.p0 / MX4_BAND) * a.k_tiles * MX4_TILE_BYTES;
+                const uint8_t* sfq = a.scales_q + (size_t)(t.q0 / MX4_BAND) * a.k_tiles * MX4_TILE_BYTES;
+                const int      row = t.group * a.np + t.p0;
+                for(int kb = kb0; kb < kb1; ++kb, ++it)
+                {
+                    const int      s  = it % STAGES;
+                    const uint32_t ph = (it / STAGES) & 1;
+                    if(!mbar_wait(empty(s), ph ^ 1, abort_flag)) { fail(0); ok = false; break; }
+                    const uint32_t st    = base + s * L::STAGE_BYTES;
+                    const uint32_t bytes = min(STAGE_TILES, a.k_tiles - kb * STAGE_TILES) * MX4_TILE_BYTES;
+                    const size_t   at    = (size_t)kb * STAGE_TILES * MX4_TILE_BYTES;
+                    mbar_arrive_expect_tx(full(s), L::P_BYTES + L::Q_BYTES + 2 * bytes);
+                    tma_load_2d(st, &map_p, kb * G_ROW_BYTES, row, full(s));
+                    tma_load_2d(st + L::P_BYTES, &map_q, kb * G_ROW_BYTES, t.q0, full(s));
+                    bulk_load(st + L::P_BYTES + L::Q_BYTES, sfp + at, bytes, full(s));
+                    bulk_load(st + L::P_BYTES + L::Q_BYTES + G_SCALE_BYTES, sfq + at, bytes, full(s));
+                }
+            }
+            if(!ok) // the copies in flight write to this CTA's shared memory
+                for(uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+                    drain_wait(full(j % STAGES), (j / STAGES) & 1);
+        }
+    }
+    else if(warp == G_MMA_WARP)
+    {
+        if(lane == 0)
+        {
+            uint32_t it = 0, chunks = 0;
+            bool     ok = true;
+            for(int tile = first; tile < total && ok; tile += stride)
+            {
+                const int q_col = tile_at<BN>(a, first_tile, tile).q0 % MX4_BAND / 32; // columns of the scale tile before Q's rows
+                for(int kb = kb0; kb < kb1; ++kb, ++it)
+                {
+                    const bool     start = (kb - kb0) % a.chunk == 0;
+                    const uint32_t buf = chunks & 1, aph = (chunks >> 1) & 1;
+                    if(start)
+                    {
+                        if(!mbar_wait(acc_empty(buf), aph ^ 1, abort_flag)) { fail(1); ok = false; break; }
+                        tc_fence_after();
+                    }
+                    const int      s  = it % STAGES;
+                    const uint32_t ph = (it / STAGES) & 1;
+                    if(!mbar_wait(full(s), ph, abort_flag)) { fail(2); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d    = tmem_base + buf * BN;
+                    const uint32_t st   = base + s * L::STAGE_BYTES;
+                    const uint32_t sp   = st + L::P_BYTES + L::Q_BYTES, sq = sp + G_SCALE_BYTES;
+                    const uint32_t tp   = tmem_base + G_SCALE_COL + 32 * s, tq = tp + 16;
+                    const int      left = a.K - kb * G_KBLOCK;
+#pragma unroll
+                    for(int i = 0; i < STAGE_TILES; ++i)
+                        if(i * 4 * mx4_block(FMT) < left)
+                        {
+                            tc_copy_scales(tp + 4 * i, scales_desc(sp + i * MX4_TILE_BYTES));
+                            tc_copy_scales(tq + 4 * i, scales_desc(sq + i * MX4_TILE_BYTES));
+                        }
+#pragma unroll
+                    for(int kk = 0; kk < G_KBLOCK / G_KSTEP; ++kk)
+                        if(kk * G_KSTEP < left)
+                        {
+                            constexpr int per  = FMT == B200_SGEMM_NVFP4 ? 1 : 2; // instructions per scale tile
+                            const uint32_t id  = kk % per * 2;                    // first byte of the scale words it takes
+                            const uint32_t off = kk * (G_KSTEP / 2);
+                            tc_mma_mx4<FMT>(d, codes_desc(st + off), codes_desc(st + L::P_BYTES + off),
+                                            mx4_idesc<FMT, BN>() | id << 4 | id << 29, tp + kk / per * 4, tq + kk / per * 4 + q_col,
+                                            !(start && kk == 0));
+                        }
+                    tc_commit(empty(s));
+                    if((kb - kb0) % a.chunk == a.chunk - 1 || kb == kb1 - 1)
+                    {
+                        tc_commit(acc_full(buf));
+                        ++chunks;
+                    }
+                }
+            }
+            if(!ok) // the products in flight write to tensor memory that is about to be freed
+            {
+                tc_commit(drained);
+                drain_wait(drained, 0);
+            }
+        }
+    }
+    else
+    {
+        const int quarter = warp & 3, half = warp >> 2;
+        uint32_t  chunks = 0;
+        bool      ok     = true;
+        const int n_chunks = (kb1 - kb0 + a.chunk - 1) / a.chunk;
+        float     factor_q = a.alpha;
+        if(a.global_q)
+            factor_q *= *a.global_q;
+        for(int tile = first; tile < total && ok; tile += stride)
+        {
+            const Tile t = tile_at<BN>(a, first_tile, tile);
+            float      acc[COLS];
+            for(int ch = 0; ch < n_chunks; ++ch, ++chunks)
+            {
+                const uint32_t buf = chunks & 1, aph = (chunks >> 1) & 1;
+                if(!mbar_wait(acc_full(buf), aph, abort_flag)) { fail(3); ok = false; break; }
+                tc_fence_after();
+                const uint32_t from = tmem_base + buf * BN + half * COLS + (uint32_t(quarter * 32) << 16);
+                constexpr int  STEP = COLS < 32 ? COLS : 32;
+#pragma unroll
+                for(int c = 0; c < COLS; c += STEP)
+                {
+                    uint32_t v[STEP];
+#pragma unroll
+                    for(int j = 0; j < STEP; j += 16)
+                        tmem_ld16(from + c + j, v + j);
+                    tmem_ld_wait();
+#pragma unroll
+                    for(int j = 0; j < STEP; ++j)
+                        acc[c + j] = ch == 0 ? __uint_as_float(v[j]) : acc[c + j] + __uint_as_float(v[j]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if(lane == 0)
+                    mbar_arrive(acc_empty(buf));
+            }
+            if(!ok)
+                break;
+            const int p = quarter * 32 + lane, q = half * COLS;
+            if(split == 1)
+            {
+                const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q;
+                store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
+            }
+            else // park the part; a cluster has one tile, so the ring is at rest
+            {
+                float* part = reinterpret_cast<float*>(ring);
+#pragma unroll
+                for(int j = 0; j < COLS; ++j)
+                    part[(q + j) * G_BP + p] = acc[j];
+            }
+        }
+    }
+
+    __syncwarp();
+    if(split > 1)
+    {
+        cluster_arrive();
+        cluster_wait();
+        if(first < total && warp < G_EPILOGUE / 32) // rank r adds and stores columns r * BN / split ..
+        {
+            const Tile  t      = tile_at<BN>(a, first_tile, first);
+            float       factor = a.alpha;
+            if(a.global_q)
+                factor *= *a.global_q;
+            if(a.global_p)
+                factor *= a.global_p[t.group];
+            const int p = threadIdx.x & (G_BP - 1), mine = BN / split;
+            for(int j = threadIdx.x / G_BP; j < mine; j += G_EPILOGUE / G_BP)
+            {
+                const int q = rank * mine + j;
+                float     sum[1] = {0.f};
+                for(int r = 0; r < split; ++r)
+                {
+                    const float v = ld_cluster(base + (uint32_t)(q * G_BP + p) * 4, r);
+                    sum[0] = r == 0 ? v : sum[0] + v;
+                }
+                if(t.q0 + q < t.q_end && t.p0 + p < a.np)
+                {
+                    const long long at = (long long)(t.p0 + p) * a.sp + (long long)(t.q0 + q) * a.sq;
+                    const float     v  = sum[0] * factor;
+                    if(a.type == B200_SGEMM_F32)
+                        static_cast<float*>(a.c)[at] = v;
+                    else if(a.type == B200_SGEMM_F16)
+                        static_cast<__half*>(a.c)[at] = from_float<__half>(v);
+                    else
+                        static_cast<__nv_bfloat16*>(a.c)[at] = from_float<__nv_bfloat16>(v);
+                }
+            }
+        }
+        cluster_arrive(); // nobody leaves while its part is being read
+        cluster_wait();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if(warp == G_MMA_WARP)
+    {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, G_TMEM_COLS);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder()
+{
+    static EncodeFn fn = [] {
+        void*                           p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess
+           || q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// rows of `pitch` code bytes; box = 128 bytes x box_rows rows, 128-byte swizzle
+bool encode_codes(CUtensorMap* map, const void* codes, size_t rows, size_t pitch, int box_rows)
+{
+    EncodeFn fn = encoder();
+    if(!fn)
+        return false;
+    const cuuint64_t dims[2]    = {(cuuint64_t)pitch, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2]     = {(cuuint32_t)G_ROW_BYTES, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2]    = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int MAX_DEVICES = 64;
+
+// SMs of the current device; also binds the device's context to this thread, which the driver's encoder needs
+int device_sms(int* sms)
+{
+    static std::atomic<int> known[MAX_DEVICES];
+    int                     device = 0;
+    cudaError_t             e      = cudaGetDevice(&device);
+    if(e != cudaSuccess)
+        return (int)e;
+    static thread_local int bound = -1;
+    if(bound != device)
+    {
+        if((e = cudaSetDevice(device)) != cudaSuccess)
+            return (int)e;
+        bound = device;
+    }
+    int n = device < MAX_DEVICES ? known[device].load(std::memory_order_relaxed) : 0;
+    if(!n)
+    {
+        if((e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess)
+            return (int)e;
+        if(device < MAX_DEVICES)
+            known[device].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return B200_SGEMM_OK;
+}
+
+struct Operand
+{
+    const void* codes;
+    const void* scales;
+    size_t      rows; // of the whole array: all groups
+};
+
+template<int FMT, int BN>
+int launch(const GArgs& a, const Operand& p, const Operand& q, size_t pitch, int grid, cudaStream_t stream)
+{
+    auto kernel = mx4_gemm_kernel<FMT, BN>;
+    using L     = GLayout<BN>;
+    CUtensorMap mp, mq;
+    if(!encode_codes(&mp, p.codes, p.rows, pitch, G_BP) || !encode_codes(&mq, q.codes, q.rows, pitch, BN))
+        return B200_SGEMM_NO_KERNEL;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM_BYTES);
+    if(e != cudaSuccess)
+        return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim            = dim3((unsigned)grid);
+    cfg.blockDim           = dim3(G_THREADS);
+    cfg.dynamicSmemBytes   = L::SMEM_BYTES;
+    cfg.stream             = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id               = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs                = attr;
+    cfg.numAttrs             = a.split > 1 ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, a, mp, mq);
+}
+
+template<int FMT>
+int launch_tile(int bn, const GArgs& a, const Operand& p, const Operand& q, size_t pitch, int grid, cudaStream_t stream)
+{
+    if(bn == 32)
+        return launch<FMT, 32>(a, p, q, pitch, grid, stream);
+    if(bn == 64)
+        return launch<FMT, 64>(a, p, q, pitch, grid, stream);
+    return launch<FMT, 128>(a, p, q, pitch, grid, stream);
+}
+
+// `a` holds what both entries agree on; `columns` is the expected number of rows of Q in a group, `tiles_q` the most column
+// tiles there can be for a tile width
+template<class TilesQ>
+int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_t columns, TilesQ tiles_q, cudaStream_t stream)
+{
+    int sms = 0, status = device_sms(&sms);
+    if(status != B200_SGEMM_OK)
+        return status;
+    a.K       = (int)K;
+    a.kblocks = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
+    a.chunk   = a.type == B200_SGEMM_F32 ? CHUNK_F32 : a.kblocks;
+    a.k_tiles = (int)mx4_tiles(format, K);
+    a.tiles_p = (a.np + G_BP - 1) / G_BP;
+    a.bands_p = a.tiles_p;
+    const int bn = columns <= 32 ? 32 : (columns <= 64 ? 64 : 128);
+    const unsigned long long tiles = (unsigned long long)a.tiles_p * tiles_q(bn);
+    if(tiles > 0x7fffffffull)
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    a.split = 1;
+    while(a.groups == 0 && a.split < 8 && tiles * a.split * 2 <= (unsigned long long)sms && a.kblocks >= a.split * 4)
+        a.split *= 2;
+    const int    grid  = a.split > 1 ? (int)tiles * a.split : (int)(tiles < (unsigned long long)sms ? tiles : sms);
+    const size_t pitch = mx4_pitch(K);
+    return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(bn, a, p, q, pitch, grid, stream)
+                                      : launch_tile<B200_SGEMM_MXFP4>(bn, a, p, q, pitch, grid, stream);
+}
+} // namespace
+
+extern "C" int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, const void* a_codes, const void* a_scales,
+                              const void* b_codes, const void* b_scales, size_t M, size_t N, size_t K, size_t ldc, float alpha,
+                              const float* global_a, const float* global_b, void* cuda_stream)
+{
+    if(!C || !a_codes || !a_scales || !b_codes || !b_scales || M == 0 || N == 0 || K == 0 || !mx4_format_ok(format)
+       || !type_ok(type_c) || layout_c & ~1)
+        return B200_SGEMM_INVALID_ARGUMENT;
+    if(M > MAX_EXTENT || N > MAX_EXTENT || K > MAX_EXTENT)
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    const bool   row = layout_c == B200_SGEMM_ROW_MAJOR;
+    const size_t packed = row ? N : M;
+    if(ldc == 0)
+        ldc = packed;
+    if(ldc < packed || misaligned(C, type_bytes(type_c)) || misaligned(a_codes, 16) || misaligned(a_scales, 16)
+       || misaligned(b_codes, 16) || misaligned(b_scales, 16) || misaligned(global_a, 4) || misaligned(global_b, 4)
+       || (format == B200_SGEMM_MXFP4 && (global_a || global_b)))
+        return B200_SGEMM_INVALID_ARGUMENT;
+    if(ldc > (size_t(1) << 40))
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    const Operand a{a_codes, a_scales, M}, b{b_codes, b_scales, N};
+    // lanes: C's contiguous dimension, unless that one is short and the other is not
+    bool b_lanes = row;
+    if(packed <= 64 && (row ? M : N) > packed)
+        b_lanes = !row;
+    GArgs g     = {};
+    g.c         = C;
+    g.sp        = b_lanes == row ? 1 : (long long)ldc;
+    g.sq        = b_lanes == row ? (long long)ldc : 1;
+    g.scales_p  = static_cast<const uint8_t*>(b_lanes ? b_scales : a_scales);
+    g.scales_q  = static_cast<const uint8_t*>(b_lanes ? a_scales : b_scales);
+    g.global_p  = b_lanes ? global_b : global_a;
+    g.global_q  = b_lanes ? global_a : global_b;
+    g.alpha     = alpha;
+    g.np        = (int)(b_lanes ? N : M);
+    g.nq        = (int)(b_lanes ? M : N);
+    g.type      = type_c;
+    const size_t nq = (size_t)g.nq;
+    return run(format, g, b_lanes ? b : a, b_lanes ? a : b, K, nq, [=](int bn) { return (nq + bn - 1) / bn; },
+               static_cast<cudaStream_t>(cuda_stream));
+}
+
+extern "C" int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
+                                      const void* b_scales, size_t rows, size_t N, size_t K, size_t ldc, size_t groups,
+                                      const int* offsets, const int* counts, size_t used_rows, float alpha,
+                                      const float* global_a, const float* global_b, void* cuda_stream)
+{
+    if(!C || !a_codes || !a_scales || !b_codes || !b_scales || !offsets || !counts || rows == 0 || N == 0 || K == 0 || groups == 0
+       || !mx4_format_ok(format) || !type_ok(type_c))
+        return B200_SGEMM_INVALID_ARGUMENT;
+    if(rows > MAX_EXTENT || N > MAX_EXTENT || K > MAX_EXTENT || groups > G_MAX_GROUPS || groups * N > MAX_EXTENT)
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    if(ldc == 0)
+        ldc = N;
+    if(ldc < N || misaligned(C, type_bytes(type_c)) || misaligned(a_codes, 16) || misaligned(a_scales, 16)
+       || misaligned(b_codes, 16) || misaligned(b_scales, 16) || misaligned(offsets, 4) || misaligned(counts, 4)
+       || misaligned(global_a, 4) || misaligned(global_b, 4) || (format == B200_SGEMM_MXFP4 && (global_a || global_b)))
+        return B200_SGEMM_INVALID_ARGUMENT;
+    if(ldc > (size_t(1) << 40))
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    GArgs g    = {};
+    g.c        = C;
+    g.sp       = 1;
+    g.sq       = (long long)ldc;
+    g.scales_p = static_cast<const uint8_t*>(b_scales);
+    g.scales_q = static_cast<const uint8_t*>(a_scales);
+    g.offsets  = offsets;
+    g.counts   = counts;
+    g.global_p = global_b;
+    g.global_q = global_a;
+    g.alpha    = alpha;
+    g.np       = (int)N;
+    g.nq       = (int)rows;
+    g.groups   = (int)groups;
+    g.type     = type_c;
+    const size_t used = used_rows && used_rows < rows ? used_rows : rows;
+    // groups start on multiples of 128 rows and so of any tile's width: no more tiles than these hold rows
+    return run(format, g, Operand{b_codes, b_scales, groups * N}, Operand{a_codes, a_scales, rows}, K, (used + groups - 1) / groups,
+               [=](int bn) { return (rows + bn - 1) / bn; }, static_cast<cudaStream_t>(cuda_stream));
+}
+
+extern "C" int b200_sgemm_mx4_device_status(int* status)
+{
+    if(!status)
+        return B200_SGEMM_INVALID_ARGUMENT;
+    cudaError_t e = cudaDeviceSynchronize();
+    if(e != cudaSuccess)
+        return (int)e;
+    const int zero = 0;
+    if((e = cudaMemcpyFromSymbol(status, g_mx4_status, sizeof(int))) != cudaSuccess)
+        return (int)e;
+    if(*status)
+        e = cudaMemcpyToSymbol(g_mx4_status, &zero, sizeof(int));
+    return (int)e;
+}

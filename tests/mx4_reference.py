@@ -1,0 +1,88 @@
+"""Microscaled 4-bit floating point in 64-bit numpy, from the definitions: what the 4-bit operators are tested against."""
+import numpy as np
+
+NVFP4, MXFP4 = 0, 1
+BLOCK = {NVFP4: 16, MXFP4: 32}
+LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+E4M3 = np.array([m * 2.0 ** -9 for m in range(8)] + [(8 + m) * 2.0 ** (e - 10) for e in range(1, 16) for m in range(8)][:-1])
+TYPE_EPS = {"f32": 2.0 ** -23, "f16": 2.0 ** -10, "bf16": 2.0 ** -7}
+
+
+def nearest(v, table):
+    """Index of the nearest entry of an ascending table; a midpoint goes to the even index."""
+    mid = (table[1:] + table[:-1]) / 2
+    below, upto = np.searchsorted(mid, v, "left"), np.searchsorted(mid, v, "right")
+    return np.where(below % 2 == 0, below, upto)
+
+
+def quantize(fmt, x, g=1.0):
+    """x [rows, K] float64 -> codes [rows, K] 0..15 and scale bytes [rows, blocks].  x / (s g): the quotient of a 24-bit
+    number and one of 28 bits; a midpoint has two bits, so 53 bits tell the three cases apart."""
+    rows, K = x.shape
+    b = BLOCK[fmt]
+    p = np.zeros((rows, -(-K // b) * b))
+    p[:, :K] = x
+    p = p.reshape(rows, -1, b)
+    bad = ~np.isfinite(p).all(-1)
+    p = np.where(bad[..., None], 0, p)
+    amax = np.abs(p).max(-1)
+    if fmt == NVFP4:
+        byte = nearest(amax / (6 * float(g)), E4M3)
+        s = E4M3[byte] * float(g)
+        byte = np.where(bad, 0x7F, byte)
+    else:
+        e = np.clip(np.frexp(amax)[1] - 3, -127, 127)
+        e = np.where(amax > 0, e, -127)
+        s, byte = 2.0 ** e, np.where(bad, 0xFF, e + 127)
+    safe = np.where(s > 0, s, 1)[..., None]
+    code = nearest(np.minimum(np.abs(p) / safe, 6), LEVELS)
+    code = np.where((s > 0)[..., None] & ~bad[..., None], code | (np.signbit(p) << 3), 0)
+    return code.reshape(rows, -1)[:, :K].astype(np.uint8), byte.astype(np.uint8)
+
+
+def pack(fmt, code, byte):
+    """The two arrays as they are stored."""
+    rows, K = code.shape
+    c = np.zeros((rows, -(-K // 32) * 32), np.uint8)
+    c[:, :K] = code
+    codes = c[:, 0::2] | c[:, 1::2] << 4
+    cols = byte.shape[1]
+    t = np.zeros((-(-rows // 128) * 128, -(-K // (4 * BLOCK[fmt])) * 4), np.uint8)
+    t[:rows, :cols] = byte
+    scales = t.reshape(-1, 4, 32, t.shape[1] // 4, 4).transpose(0, 3, 2, 1, 4)
+    return codes.reshape(-1).copy(), scales.reshape(-1).copy()
+
+
+def unpack(fmt, codes, scales, rows, K):
+    """codes and scale bytes by the address that the format gives them."""
+    pitch, b = -(-K // 32) * 16, BLOCK[fmt]
+    k = np.arange(K)
+    code = codes.reshape(rows, pitch)[:, k // 2] >> (k % 2 * 4) & 15
+    r, c = np.arange(rows)[:, None], np.arange(-(-K // b))[None]
+    tiles = -(-K // (4 * b))
+    byte = scales[(r // 128 * tiles + c // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + c % 4]
+    return code, byte
+
+
+def values(fmt, code, byte, g=1.0):
+    """float64 values of codes [rows, K] and scale bytes."""
+    if fmt == NVFP4:
+        s = np.where((byte & 0x7F) == 0x7F, np.nan, E4M3[np.minimum(byte, 0x7E)])
+    else:
+        s = np.where(byte == 0xFF, np.nan, 2.0 ** (byte.astype(np.float64) - 127))
+    s = np.repeat(s, BLOCK[fmt], 1)[:, :code.shape[1]]
+    return np.where(code >= 8, -1.0, 1.0) * LEVELS[code & 7] * s * float(g)
+
+
+def product_bound(a, b, ref, dtype, chunk=None):
+    """How far a product may be from `ref` = a @ b.T.  The tensor core adds the 64 products of an instruction and its
+    accumulator by aligning and cutting off: 2^-22 of the sum of magnitudes for each instruction, taken over all of K or,
+    for FP32 results, over 512 k, whose sums are then added with 2^-24 each.  Two roundings of the factor, one of its
+    product and one of the result; FP16's subnormals have 2^-25."""
+    K = a.shape[1]
+    size = np.abs(a) @ np.abs(b).T
+    steps = -(-K // 64)
+    inside = min(steps, 8) if dtype == "f32" else steps
+    err = size * (inside * 2.0 ** -22 + (-(-K // 512) * 2.0 ** -24 if dtype == "f32" else 0))
+    err += np.abs(ref) * (4 * 2.0 ** -24 + TYPE_EPS[dtype] / 2)
+    return err + (2.0 ** -25 if dtype == "f16" else 0) + 1e-300
