@@ -9,16 +9,20 @@
 //            that is the weights, and the tokens cost BN = 32 columns instead of a tile of 128 rows
 //   columns  the other one; the rows of the groups in the grouped product
 //
+// Tiles.  128 lanes x 32, 64 or 128 columns by one CTA, or 256 lanes x 128 or 256 columns by a pair of CTAs on
+// neighbouring SMs: each holds 128 of the lanes, half of Q's rows and all of Q's scales, and the first one issues for both.
+// A pair reads half of Q from the L2 and from shared memory and issues half the scale copies per product.
+//
 // One persistent CTA per SM, 10 warps:
 //   warps 0-7  accumulate and store.  The tensor core adds into its FP32 accumulator with truncation, so for an FP32
 //              result the accumulator is emptied into registers every CHUNK_F32 K blocks and the parts are added there,
-//              rounded to nearest; results of 16 bits keep one accumulator for the whole of K (the bias, measured below
-//              1e-5 of the result at K = 16384, is a hundredth of their rounding).
-//   warp 8     one thread fetches the stages: the two operands' codes by TMA (256 k = 128-byte rows, 128-byte swizzle; zero
-//              beyond the matrix), the scale tiles as they lie by bulk copies
-//   warp 9     one thread copies the stage's scale tiles into tensor memory (tcgen05.cp, replicated to the four lane
-//              quarters) and issues the products, 64 k each.  Scales go to a tensor-memory slot of the stage's own, which is
-//              free as soon as the stage is.
+//              rounded to nearest; results of 16 bits keep one accumulator for the whole of K (a bias of at most 2^-23 a
+//              product of 64 k is below their rounding up to K = 2^18).
+//   warp 8     fetches the stages by TMA: the two operands' codes (256 k = rows of 128 bytes, 128-byte swizzle) and the scale
+//              tiles as they lie; zero beyond the matrix
+//   warp 9     copies the stage's scale tiles into tensor memory (tcgen05.cp, replicated to the four lane quarters) and issues
+//              the products, 64 k each.  Scales go to a tensor-memory slot of the stage's own, which is free as soon as the
+//              stage is.
 // Few tiles: a cluster of 2, 4 or 8 CTAs shares a tile, each with a range of K of its own; the parts meet through
 // distributed shared memory and are added in ascending order of K, so the result does not depend on timing and no
 // workspace is needed (a captured graph can be replayed on any stream).
@@ -35,46 +39,55 @@ namespace
 {
 using namespace sgemm_b200;
 
-constexpr int G_BP        = 128; // lane tile
-constexpr int G_KBLOCK    = 256; // k of one stage: a 128-byte row of codes
-constexpr int G_ROW_BYTES = G_KBLOCK / 2;
-constexpr int G_KSTEP     = 64; // k of one instruction
-constexpr int G_EPILOGUE  = 256;
-constexpr int G_TMA_WARP  = 8;
-constexpr int G_MMA_WARP  = 9;
-constexpr int G_THREADS   = 320;
-constexpr int G_TMEM_COLS = 512;
-constexpr int G_SCALE_COL = 256; // tensor-memory columns 0..255: two accumulators, then 32 of scales per stage
+constexpr int G_LANES      = 128; // lanes of a CTA
+constexpr int G_KBLOCK     = 256; // k of one stage: a 128-byte row of codes
+constexpr int G_ROW_BYTES  = G_KBLOCK / 2;
+constexpr int G_KSTEP      = 64; // k of one instruction
+constexpr int G_EPILOGUE   = 256;
+constexpr int G_TMA_WARP   = 8;
+constexpr int G_MMA_WARP   = 9;
+constexpr int G_THREADS    = 320;
+constexpr int G_TMEM_COLS  = 512;
+constexpr int G_SCALE_COL  = 256; // tensor-memory columns 0..255: accumulators; behind them a slot of scales per stage
 constexpr int G_MAX_GROUPS = 1024;
-constexpr int CHUNK_F32   = 2;  // K blocks (512 k, 8 products) added inside the tensor core for an FP32 result
-constexpr int G_SCALE_BYTES = 4 * MX4_TILE_BYTES; // of one operand in a stage
+constexpr int CHUNK_F32    = 2; // K blocks (512 k, 8 products) added inside the tensor core for an FP32 result
 
 constexpr int G_ERR_WAIT  = 1; // status bits: a wait gave up (bits 8.. say which);
 constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the matrix, the group was left out
 
 __device__ int g_mx4_status;
 
-template<int BN>
+// PAIR: CTAs that share a tile's instructions
+template<int FMT, int BN, int PAIR>
 struct GLayout
 {
-    static constexpr int    P_BYTES     = G_BP * G_ROW_BYTES;
-    static constexpr int    Q_BYTES     = BN * G_ROW_BYTES;
-    static constexpr int    STAGE_BYTES = P_BYTES + Q_BYTES + 2 * G_SCALE_BYTES;
-    static constexpr int    STAGES      = BN == 128 ? 6 : (BN == 64 ? 7 : 8);
+    static constexpr int    TILE_P      = PAIR * G_LANES;
+    static constexpr int    Q_ROWS      = BN / PAIR;                     // of this CTA
+    static constexpr int    Q_BANDS     = (BN + MX4_BAND - 1) / MX4_BAND; // bands of scales that a column tile touches
+    static constexpr int    TILES       = G_KBLOCK / (4 * mx4_block(FMT)); // scale tiles of a band in a stage
+    static constexpr int    P_BYTES     = G_LANES * G_ROW_BYTES;
+    static constexpr int    Q_BYTES     = Q_ROWS * G_ROW_BYTES;
+    static constexpr int    P_SCALES    = TILES * MX4_TILE_BYTES;
+    static constexpr int    Q_SCALES    = Q_BANDS * P_SCALES;
+    static constexpr int    FILL_BYTES  = P_BYTES + Q_BYTES + P_SCALES + Q_SCALES;
+    static constexpr int    STAGE_BYTES = (FILL_BYTES + 1023) / 1024 * 1024;
+    static constexpr int    SLOT_COLS   = 4 * TILES * (1 + Q_BANDS); // tensor-memory columns of a stage's scales
+    static constexpr int    BY_SMEM     = (216 * 1024) / STAGE_BYTES;
+    static constexpr int    BY_TMEM     = (G_TMEM_COLS - G_SCALE_COL) / SLOT_COLS;
+    static constexpr int    STAGES      = BY_SMEM < BY_TMEM ? (BY_SMEM < 8 ? BY_SMEM : 8) : (BY_TMEM < 8 ? BY_TMEM : 8);
+    static constexpr int    ACCS        = BN > 128 ? 1 : 2; // accumulators
     static constexpr int    BARRIERS    = 2 * STAGES + 5;
     static constexpr size_t SMEM_BYTES  = size_t(STAGES) * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers, misc*/;
     static_assert(8 * BARRIERS + 16 <= 256, "barrier area");
-    static_assert(STAGE_BYTES % 1024 == 0, "swizzled tiles start on 1024 bytes");
-    static_assert(STAGES * 32 + G_SCALE_COL <= G_TMEM_COLS && 2 * BN <= G_SCALE_COL, "tensor memory");
-    static_assert(BN * G_BP * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile lie in the ring");
+    static_assert(ACCS * BN <= G_SCALE_COL, "tensor memory");
+    static_assert(SMEM_BYTES + (G_MAX_GROUPS + 1) * 4 <= 227 * 1024, "shared memory");
+    static_assert(PAIR > 1 || BN * G_LANES * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile lie in the ring");
 };
 
 struct GArgs
 {
     void*          c;
     long long      sp, sq; // element strides of C along lanes and columns; one of them is 1
-    const uint8_t* scales_p;
-    const uint8_t* scales_q;
     const int*     offsets; // grouped: first row (of Q and C) of each group, and rows
     const int*     counts;
     const float*   global_p;
@@ -83,40 +96,62 @@ struct GArgs
     int            np;      // lane extent (of one group's operand)
     int            nq;      // column extent: rows of Q
     int            K, kblocks, chunk;
-    int            k_tiles; // scale tiles along k
-    int            tiles_p, bands_p;
+    int            tiles_p, bands_p; // lane tiles; bands of scales of one group's P
     int            groups;  // 0: one product
     int            split;   // CTAs of a cluster that share a tile
     int            type;
 };
 
 // ---- instructions ----------------------------------------------------------------------------------------
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+// tile copies that signal a barrier of the pair's first CTA; `bar` as a cluster address
+template<int PAIR>
+__device__ __forceinline__ void load_codes(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar)
 {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+    if constexpr(PAIR == 1)
+        tma_load_2d(dst, map, c0, c1, bar);
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+                     : "memory");
 }
-// a scale tile (32 rows of 16 bytes) to four columns of all four lane quarters
+template<int PAIR>
+__device__ __forceinline__ void load_scales(uint32_t dst, const CUtensorMap* map, int tile, int band, uint32_t bar)
+{
+    if constexpr(PAIR == 1)
+        tma_load_3d(dst, map, 0, tile, band, bar);
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(tile), "r"(band), "r"(bar)
+                     : "memory");
+}
+// a scale tile (32 rows of 16 bytes) to four columns of all four lane quarters; a pair: each CTA its own tile
+template<int PAIR>
 __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc)
 {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if constexpr(PAIR == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template<int FMT>
+#define MX4_MMA(GROUP, VEC)                                                                                                      \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                              \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::mxf4nvf4.block_scale.scale_vec::" VEC " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" \
+                 ::"r"(d), "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(sf_p), "r"(sf_q), "r"(accumulate)                            \
+                 : "memory")
+template<int FMT, int PAIR>
 __device__ __forceinline__ void tc_mma_mx4(uint32_t d, uint64_t p_desc, uint64_t q_desc, uint32_t idesc, uint32_t sf_p, uint32_t sf_q,
                                            uint32_t accumulate)
 {
-    if(FMT == B200_SGEMM_NVFP4)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(sf_p), "r"(sf_q), "r"(accumulate)
-                     : "memory");
+    if constexpr(FMT == B200_SGEMM_NVFP4 && PAIR == 1)
+        MX4_MMA("1", "4X");
+    else if constexpr(FMT == B200_SGEMM_NVFP4)
+        MX4_MMA("2", "4X");
+    else if constexpr(PAIR == 1)
+        MX4_MMA("1", "2X");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(sf_p), "r"(sf_q), "r"(accumulate)
-                     : "memory");
+        MX4_MMA("2", "2X");
 }
+#undef MX4_MMA
 // codes: rows of 128 bytes with the 128-byte swizzle, 1024 bytes between groups of eight rows
 __device__ __forceinline__ uint64_t codes_desc(uint32_t addr)
 {
@@ -130,27 +165,50 @@ __device__ __forceinline__ uint64_t scales_desc(uint32_t addr)
 }
 // block-scaled product: e2m1 operands (1), both K-major, N >> 3, scale type (0 e4m3, 1 e8m0), M >> 4; which bytes of the
 // 32-bit scale words an instruction takes is added by the issuer (bits 4-5 for Q, 29-30 for P)
-template<int FMT, int BN>
+template<int FMT, int BN, int PAIR>
 __device__ __forceinline__ constexpr uint32_t mx4_idesc()
 {
     return (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (FMT == B200_SGEMM_MXFP4 ? 1u << 23 : 0u)
-           | (uint32_t(G_BP >> 4) << 24);
+           | (uint32_t(PAIR * G_LANES >> 4) << 24);
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank)
+// the address in CTA `rank` of the cluster that corresponds to `addr` here
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank)
 {
     uint32_t at;
-    float    v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return at;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(addr, rank)) : "memory");
     return v;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // what is in flight when a CTA gives up has to land before it leaves; bounded, without looking at the abort flag
 __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity)
 {
     const uint64_t t0 = global_timer_ns();
     while(!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < 100ull * 1000 * 1000) {}
+}
+
+// one thread of a converged warp
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// a bounded wait of a whole warp: all lanes see the same outcome
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag)
+{
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------------
@@ -160,18 +218,18 @@ struct Tile
 };
 // one product: bands of 16 lane tiles, columns advancing inside a band, so that CTAs running together share operands in
 // the L2; groups: all lane tiles of a group's column tile, then the next column tile, so a group's weights stay in the L2
-template<int BN>
+template<int BN, int TILE_P>
 __device__ __forceinline__ Tile tile_at(const GArgs& a, const int* first_tile, int tile)
 {
     Tile t;
     if(a.groups == 0)
     {
-        constexpr int BAND = 16;
+        constexpr int BAND = 16 * G_LANES / TILE_P;
         const int tiles_q = (a.nq + BN - 1) / BN;
         const int band = tile / (BAND * tiles_q), in = tile - band * BAND * tiles_q;
         const int wide = min(BAND, a.tiles_p - band * BAND);
         t.group = 0;
-        t.p0    = (band * BAND + in % wide) * G_BP;
+        t.p0    = (band * BAND + in % wide) * TILE_P;
         t.q0    = in / wide * BN;
         t.q_end = a.nq;
         return t;
@@ -188,7 +246,7 @@ __device__ __forceinline__ Tile tile_at(const GArgs& a, const int* first_tile, i
     }
     const int off = a.offsets[lo];
     t.group = lo;
-    t.p0    = (tile - qt * a.tiles_p) * G_BP;
+    t.p0    = (tile - qt * a.tiles_p) * TILE_P;
     t.q0    = off + (qt - first_tile[lo]) * BN;
     t.q_end = off + a.counts[lo];
     return t;
@@ -241,14 +299,60 @@ __device__ __forceinline__ void store_typed(const GArgs& a, const float (&acc)[C
         store_columns<__nv_bfloat16>(a, acc, factor, p, q0, q_end);
 }
 
-template<int FMT, int BN>
-__global__ void __launch_bounds__(G_THREADS, 1)
-    mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q)
+struct Maps
 {
-    using L = GLayout<BN>;
-    constexpr int STAGES      = L::STAGES;
-    constexpr int STAGE_TILES = G_KBLOCK / (4 * mx4_block(FMT)); // scale tiles of a stage, per operand
-    constexpr int COLS        = BN / 2;                          // columns of one epilogue thread
+    CUtensorMap p, q, scales_p, scales_q;
+};
+
+// two results of 16 bits as they are stored, the first in the lower half
+__device__ __forceinline__ uint32_t pack16(int type, float x, float y)
+{
+    if(type == B200_SGEMM_F16)
+    {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template<int COLS>
+__device__ __forceinline__ void store_packed(const GArgs& a, const uint32_t (&v)[COLS / 2], int p, int q0, int q_end)
+{
+    if(p >= a.np)
+        return;
+    uint16_t* c = static_cast<uint16_t*>(a.c) + (long long)p * a.sp + (long long)q0 * a.sq;
+    if(a.sq == 1)
+    {
+        const bool vector = (reinterpret_cast<uintptr_t>(c) & 15) == 0;
+#pragma unroll
+        for(int j = 0; j < COLS; j += 8)
+        {
+            if(vector && q0 + j + 8 <= q_end)
+                *reinterpret_cast<uint4*>(c + j) = make_uint4(v[j / 2], v[j / 2 + 1], v[j / 2 + 2], v[j / 2 + 3]);
+            else
+            {
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    if(q0 + j + i < q_end)
+                        c[j + i] = (uint16_t)(v[(j + i) / 2] >> (16 * (i & 1)));
+            }
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int j = 0; j < COLS; ++j)
+            if(q0 + j < q_end)
+                c[(long long)j * a.sq] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+    }
+}
+
+template<int FMT, int BN, int PAIR>
+__global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ Maps maps)
+{
+    using L = GLayout<FMT, BN, PAIR>;
+    constexpr int STAGES = L::STAGES;
+    constexpr int COLS   = BN / 2; // columns of one epilogue thread
     extern __shared__ uint8_t smem_raw[];
     __shared__ int first_tile[G_MAX_GROUPS + 1];
     const uint32_t raw_addr = (uint32_t)__cvta_generic_to_shared(smem_raw);
@@ -264,7 +368,10 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     uint32_t*      tmem_slot  = reinterpret_cast<uint32_t*>(misc);
     volatile int*  abort_flag = reinterpret_cast<volatile int*>(misc + 8);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int split = a.split, shared_by = PAIR * split; // CTAs of the cluster
+    const int rank  = shared_by > 1 ? (int)(blockIdx.x % shared_by) : 0;
+    const int lane0 = PAIR > 1 ? rank * G_LANES : 0; // this CTA's first lane in the tile
     if(threadIdx.x == 0)
     {
         for(int s = 0; s < STAGES; ++s)
@@ -275,7 +382,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         for(int b = 0; b < 2; ++b)
         {
             mbar_init(acc_full(b), 1);
-            mbar_init(acc_empty(b), G_EPILOGUE / 32);
+            mbar_init(acc_empty(b), PAIR * G_EPILOGUE / 32);
         }
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -283,8 +390,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     }
     if(warp == G_MMA_WARP)
     {
-        tmem_alloc((uint32_t)__cvta_generic_to_shared(tmem_slot), G_TMEM_COLS);
-        tmem_relinquish();
+        tmem_alloc<PAIR>((uint32_t)__cvta_generic_to_shared(tmem_slot), G_TMEM_COLS);
+        tmem_relinquish<PAIR>();
     }
     if(warp == G_TMA_WARP && a.groups) // column tiles before each group
     {
@@ -318,13 +425,18 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if(PAIR > 1) // the other CTA's barriers and tensor memory are there
+    {
+        cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const int split = a.split, rank = split > 1 ? (int)(blockIdx.x % split) : 0;
-    const int first = blockIdx.x / split, stride = gridDim.x / split;
+    const int first = blockIdx.x / shared_by, stride = gridDim.x / shared_by;
     const int total = (a.groups ? first_tile[a.groups] : (a.nq + BN - 1) / BN) * a.tiles_p;
-    const int kb0 = (int)((long long)a.kblocks * rank / split), kb1 = (int)((long long)a.kblocks * (rank + 1) / split);
+    const int part  = PAIR > 1 ? 0 : rank; // this CTA's range of K
+    const int kb0 = (int)((long long)a.kblocks * part / split), kb1 = (int)((long long)a.kblocks * (part + 1) / split);
     // the first wait of the CTA that gives up records where (bits 8..) and raises the abort flag for the others
     auto fail = [&](int where) {
         if(atomicExch(const_cast<int*>(abort_flag), 1) == 0)
@@ -333,100 +445,118 @@ __global__ void __launch_bounds__(G_THREADS, 1)
 
     if(warp == G_TMA_WARP)
     {
-        if(lane == 0)
+        // here and below the whole warp walks the loop, so that addresses and descriptors are uniform, and one thread
+        // issues: with the loop inside `if(lane == 0)` the compiler moved every operand of every instruction to the uniform
+        // registers as if lanes could differ, and the 8192 cube took 680 us instead of 285
+        const bool issuer = elect_one();
+        uint32_t   s = 0, ph = 0;
+        bool       ok = true;
+        for(int tile = first; tile < total && ok; tile += stride)
         {
-            uint32_t it = 0;
-            bool     ok = true;
-            for(int tile = first; tile < total && ok; tile += stride)
+            const Tile t    = tile_at<BN, L::TILE_P>(a, first_tile, tile);
+            const int  row  = t.group * a.np + t.p0 + lane0, q_row = t.q0 + (PAIR > 1 ? rank * L::Q_ROWS : 0);
+            const int  band = t.group * a.bands_p + (t.p0 + lane0) / MX4_BAND;
+            for(int kb = kb0; kb < kb1; ++kb)
             {
-                const Tile     t   = tile_at<BN>(a, first_tile, tile);
-                const uint8_t* sfp = a.scales_p + (size_t)(t.group * a.bands_p + t.p0 / MX4_BAND) * a.k_tiles * MX4_TILE_BYTES;
-                const uint8_t* sfq = a.scales_q + (size_t)(t.q0 / MX4_BAND) * a.k_tiles * MX4_TILE_BYTES;
-                const int      row = t.group * a.np + t.p0;
-                for(int kb = kb0; kb < kb1; ++kb, ++it)
+                if(!warp_wait(empty(s), ph ^ 1, abort_flag)) { fail(0); ok = false; break; }
+                if(issuer)
                 {
-                    const int      s  = it % STAGES;
-                    const uint32_t ph = (it / STAGES) & 1;
-                    if(!mbar_wait(empty(s), ph ^ 1, abort_flag)) { fail(0); ok = false; break; }
-                    const uint32_t st    = base + s * L::STAGE_BYTES;
-                    const uint32_t bytes = min(STAGE_TILES, a.k_tiles - kb * STAGE_TILES) * MX4_TILE_BYTES;
-                    const size_t   at    = (size_t)kb * STAGE_TILES * MX4_TILE_BYTES;
-                    mbar_arrive_expect_tx(full(s), L::P_BYTES + L::Q_BYTES + 2 * bytes);
-                    tma_load_2d(st, &map_p, kb * G_ROW_BYTES, row, full(s));
-                    tma_load_2d(st + L::P_BYTES, &map_q, kb * G_ROW_BYTES, t.q0, full(s));
-                    bulk_load(st + L::P_BYTES + L::Q_BYTES, sfp + at, bytes, full(s));
-                    bulk_load(st + L::P_BYTES + L::Q_BYTES + G_SCALE_BYTES, sfq + at, bytes, full(s));
+                    const uint32_t st  = base + s * L::STAGE_BYTES;
+                    const uint32_t bar = PAIR > 1 ? cluster_addr(full(s), 0) : full(s);
+                    if(rank == 0 || PAIR == 1)
+                        mbar_arrive_expect_tx(full(s), PAIR * L::FILL_BYTES);
+                    load_codes<PAIR>(st, &maps.p, kb * G_ROW_BYTES, row, bar);
+                    load_codes<PAIR>(st + L::P_BYTES, &maps.q, kb * G_ROW_BYTES, q_row, bar);
+                    load_scales<PAIR>(st + L::P_BYTES + L::Q_BYTES, &maps.scales_p, kb * L::TILES, band, bar);
+                    load_scales<PAIR>(st + L::P_BYTES + L::Q_BYTES + L::P_SCALES, &maps.scales_q, kb * L::TILES, t.q0 / MX4_BAND, bar);
+                }
+                __syncwarp();
+                if(++s == STAGES)
+                {
+                    s = 0;
+                    ph ^= 1;
                 }
             }
-            if(!ok) // the copies in flight write to this CTA's shared memory
-                for(uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
-                    drain_wait(full(j % STAGES), (j / STAGES) & 1);
         }
+        // the copies in flight write to shared memory of this CTA (and of its pair, which stays until the end of both): wait
+        // for each stage's last fill, if it had one
+        if(!ok && (PAIR == 1 || rank == 0))
+            for(int j = 0; j < STAGES; ++j)
+            {
+                const uint32_t fill = j < (int)s ? ph : ph ^ 1; // parity of the fill before the one that would come next
+                drain_wait(full(j), fill);
+            }
     }
     else if(warp == G_MMA_WARP)
     {
-        if(lane == 0)
+        const bool issuer = elect_one();
+        uint32_t   s = 0, ph = 0, buf = 0, acc_ph = 0;
+        bool       ok = true;
+        for(int tile = first; tile < total && ok && (PAIR == 1 || rank == 0); tile += stride)
         {
-            uint32_t it = 0, chunks = 0;
-            bool     ok = true;
-            for(int tile = first; tile < total && ok; tile += stride)
+            const uint32_t q_col   = tile_at<BN, L::TILE_P>(a, first_tile, tile).q0 % MX4_BAND / 32; // columns of the scale tile before Q's rows
+            int            in_chunk = 0;
+            for(int kb = kb0; kb < kb1; ++kb)
             {
-                const int q_col = tile_at<BN>(a, first_tile, tile).q0 % MX4_BAND / 32; // columns of the scale tile before Q's rows
-                for(int kb = kb0; kb < kb1; ++kb, ++it)
+                if(in_chunk == 0 && !warp_wait(acc_empty(buf), acc_ph ^ 1, abort_flag)) { fail(1); ok = false; break; }
+                if(!warp_wait(full(s), ph, abort_flag)) { fail(2); ok = false; break; }
+                tc_fence_after();
+                const bool last = in_chunk == a.chunk - 1 || kb == kb1 - 1;
+                if(issuer)
                 {
-                    const bool     start = (kb - kb0) % a.chunk == 0;
-                    const uint32_t buf = chunks & 1, aph = (chunks >> 1) & 1;
-                    if(start)
-                    {
-                        if(!mbar_wait(acc_empty(buf), aph ^ 1, abort_flag)) { fail(1); ok = false; break; }
-                        tc_fence_after();
-                    }
-                    const int      s  = it % STAGES;
-                    const uint32_t ph = (it / STAGES) & 1;
-                    if(!mbar_wait(full(s), ph, abort_flag)) { fail(2); ok = false; break; }
-                    tc_fence_after();
                     const uint32_t d    = tmem_base + buf * BN;
                     const uint32_t st   = base + s * L::STAGE_BYTES;
-                    const uint32_t sp   = st + L::P_BYTES + L::Q_BYTES, sq = sp + G_SCALE_BYTES;
-                    const uint32_t tp   = tmem_base + G_SCALE_COL + 32 * s, tq = tp + 16;
+                    const uint32_t tp   = tmem_base + G_SCALE_COL + L::SLOT_COLS * s, tq = tp + 4 * L::TILES;
+                    const uint64_t sp   = scales_desc(st + L::P_BYTES + L::Q_BYTES), sq = sp + (L::P_SCALES >> 4);
+                    const uint64_t dp   = codes_desc(st), dq = dp + (L::P_BYTES >> 4);
                     const int      left = a.K - kb * G_KBLOCK;
 #pragma unroll
-                    for(int i = 0; i < STAGE_TILES; ++i)
+                    for(int i = 0; i < L::TILES; ++i)
                         if(i * 4 * mx4_block(FMT) < left)
                         {
-                            tc_copy_scales(tp + 4 * i, scales_desc(sp + i * MX4_TILE_BYTES));
-                            tc_copy_scales(tq + 4 * i, scales_desc(sq + i * MX4_TILE_BYTES));
+                            tc_copy_scales<PAIR>(tp + 4 * i, sp + i * (MX4_TILE_BYTES >> 4));
+#pragma unroll
+                            for(int b = 0; b < L::Q_BANDS; ++b) // an instruction takes the columns of all bands in a row
+                                tc_copy_scales<PAIR>(tq + 4 * (i * L::Q_BANDS + b), sq + (b * L::TILES + i) * (MX4_TILE_BYTES >> 4));
                         }
 #pragma unroll
                     for(int kk = 0; kk < G_KBLOCK / G_KSTEP; ++kk)
                         if(kk * G_KSTEP < left)
                         {
-                            constexpr int per  = FMT == B200_SGEMM_NVFP4 ? 1 : 2; // instructions per scale tile
+                            constexpr int  per = FMT == B200_SGEMM_NVFP4 ? 1 : 2; // instructions per scale tile
                             const uint32_t id  = kk % per * 2;                    // first byte of the scale words it takes
-                            const uint32_t off = kk * (G_KSTEP / 2);
-                            tc_mma_mx4<FMT>(d, codes_desc(st + off), codes_desc(st + L::P_BYTES + off),
-                                            mx4_idesc<FMT, BN>() | id << 4 | id << 29, tp + kk / per * 4, tq + kk / per * 4 + q_col,
-                                            !(start && kk == 0));
+                            constexpr int  off = G_KSTEP / 2 >> 4;
+                            tc_mma_mx4<FMT, PAIR>(d, dp + kk * off, dq + kk * off, mx4_idesc<FMT, BN, PAIR>() | id << 4 | id << 29,
+                                                  tp + kk / per * 4, tq + kk / per * 4 * L::Q_BANDS + q_col, in_chunk > 0 || kk > 0);
                         }
-                    tc_commit(empty(s));
-                    if((kb - kb0) % a.chunk == a.chunk - 1 || kb == kb1 - 1)
-                    {
-                        tc_commit(acc_full(buf));
-                        ++chunks;
-                    }
+                    tc_commit<PAIR>(empty(s));
+                    if(last)
+                        tc_commit<PAIR>(acc_full(buf));
+                }
+                __syncwarp();
+                in_chunk = last ? 0 : in_chunk + 1;
+                if(last && ++buf == L::ACCS)
+                {
+                    buf = 0;
+                    acc_ph ^= 1;
+                }
+                if(++s == STAGES)
+                {
+                    s = 0;
+                    ph ^= 1;
                 }
             }
-            if(!ok) // the products in flight write to tensor memory that is about to be freed
-            {
-                tc_commit(drained);
-                drain_wait(drained, 0);
-            }
+        }
+        if(!ok && issuer) // the products in flight write to tensor memory that is about to be freed
+        {
+            tc_commit<PAIR>(drained);
+            drain_wait(drained, 0);
         }
     }
     else
     {
         const int quarter = warp & 3, half = warp >> 2;
-        uint32_t  chunks = 0;
+        uint32_t  buf = 0, acc_ph = 0;
         bool      ok     = true;
         const int n_chunks = (kb1 - kb0 + a.chunk - 1) / a.chunk;
         float     factor_q = a.alpha;
@@ -434,71 +564,108 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             factor_q *= *a.global_q;
         for(int tile = first; tile < total && ok; tile += stride)
         {
-            const Tile t = tile_at<BN>(a, first_tile, tile);
-            float      acc[COLS];
-            for(int ch = 0; ch < n_chunks; ++ch, ++chunks)
+            const Tile t = tile_at<BN, L::TILE_P>(a, first_tile, tile);
+            if constexpr(L::ACCS == 1) // results of 16 bits: rounded into registers, so that the one accumulator is free at once
             {
-                const uint32_t buf = chunks & 1, aph = (chunks >> 1) & 1;
-                if(!mbar_wait(acc_full(buf), aph, abort_flag)) { fail(3); ok = false; break; }
+                const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q;
+                uint32_t    out[COLS / 2];
+                if(!warp_wait(acc_full(0), acc_ph, abort_flag)) { fail(3); ok = false; break; }
                 tc_fence_after();
-                const uint32_t from = tmem_base + buf * BN + half * COLS + (uint32_t(quarter * 32) << 16);
-                constexpr int  STEP = COLS < 32 ? COLS : 32;
+                const uint32_t from = tmem_base + half * COLS + (uint32_t(quarter * 32) << 16);
 #pragma unroll
-                for(int c = 0; c < COLS; c += STEP)
+                for(int c = 0; c < COLS; c += 32)
                 {
-                    uint32_t v[STEP];
-#pragma unroll
-                    for(int j = 0; j < STEP; j += 16)
-                        tmem_ld16(from + c + j, v + j);
+                    uint32_t v[32];
+                    tmem_ld32(from + c, v);
                     tmem_ld_wait();
 #pragma unroll
-                    for(int j = 0; j < STEP; ++j)
-                        acc[c + j] = ch == 0 ? __uint_as_float(v[j]) : acc[c + j] + __uint_as_float(v[j]);
+                    for(int j = 0; j < 32; j += 2)
+                        out[(c + j) / 2] = pack16(a.type, __uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if(lane == 0)
-                    mbar_arrive(acc_empty(buf));
+                    mbar_arrive_cluster(cluster_addr(acc_empty(0), 0));
+                acc_ph ^= 1;
+                store_packed<COLS>(a, out, t.p0 + lane0 + quarter * 32 + lane, t.q0 + half * COLS, t.q_end);
+                continue;
             }
-            if(!ok)
-                break;
-            const int p = quarter * 32 + lane, q = half * COLS;
-            if(split == 1)
+            else
             {
-                const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q;
-                store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
-            }
-            else // park the part; a cluster has one tile, so the ring is at rest
-            {
-                float* part = reinterpret_cast<float*>(ring);
-#pragma unroll
-                for(int j = 0; j < COLS; ++j)
-                    part[(q + j) * G_BP + p] = acc[j];
+                float acc[COLS];
+                for(int ch = 0; ch < n_chunks; ++ch)
+                {
+                    if(!warp_wait(acc_full(buf), acc_ph, abort_flag)) { fail(3); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t from = tmem_base + buf * BN + half * COLS + (uint32_t(quarter * 32) << 16);
+                    constexpr int  STEP = COLS < 32 ? COLS : 32;
+    #pragma unroll
+                    for(int c = 0; c < COLS; c += STEP)
+                    {
+                        uint32_t v[STEP];
+    #pragma unroll
+                        for(int j = 0; j < STEP; j += 16)
+                            tmem_ld16(from + c + j, v + j);
+                        tmem_ld_wait();
+    #pragma unroll
+                        for(int j = 0; j < STEP; ++j)
+                            acc[c + j] = ch == 0 ? __uint_as_float(v[j]) : acc[c + j] + __uint_as_float(v[j]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if(lane == 0)
+                    {
+                        if(PAIR > 1)
+                            mbar_arrive_cluster(cluster_addr(acc_empty(buf), 0));
+                        else
+                            mbar_arrive(acc_empty(buf));
+                    }
+                    if(++buf == L::ACCS)
+                    {
+                        buf = 0;
+                        acc_ph ^= 1;
+                    }
+                }
+                if(!ok)
+                    break;
+                const int p = lane0 + quarter * 32 + lane, q = half * COLS;
+                if(PAIR > 1 || split == 1)
+                {
+                    const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q;
+                    store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
+                }
+                else // park the part; a cluster has one tile, so the ring is at rest
+                {
+                    float* part = reinterpret_cast<float*>(ring);
+    #pragma unroll
+                    for(int j = 0; j < COLS; ++j)
+                        part[(q + j) * G_LANES + p] = acc[j];
+                }
             }
         }
     }
 
     __syncwarp();
-    if(split > 1)
+    if(PAIR == 1 && split > 1)
     {
         cluster_arrive();
         cluster_wait();
         if(first < total && warp < G_EPILOGUE / 32) // rank r adds and stores columns r * BN / split ..
         {
-            const Tile  t      = tile_at<BN>(a, first_tile, first);
+            const Tile  t      = tile_at<BN, L::TILE_P>(a, first_tile, first);
             float       factor = a.alpha;
             if(a.global_q)
                 factor *= *a.global_q;
             if(a.global_p)
                 factor *= a.global_p[t.group];
-            const int p = threadIdx.x & (G_BP - 1), mine = BN / split;
-            for(int j = threadIdx.x / G_BP; j < mine; j += G_EPILOGUE / G_BP)
+            const int p = threadIdx.x & (G_LANES - 1), mine = BN / split;
+            for(int j = threadIdx.x / G_LANES; j < mine; j += G_EPILOGUE / G_LANES)
             {
                 const int q = rank * mine + j;
                 float     sum[1] = {0.f};
                 for(int r = 0; r < split; ++r)
                 {
-                    const float v = ld_cluster(base + (uint32_t)(q * G_BP + p) * 4, r);
+                    const float v = ld_cluster(base + (uint32_t)(q * G_LANES + p) * 4, r);
                     sum[0] = r == 0 ? v : sum[0] + v;
                 }
                 if(t.q0 + q < t.q_end && t.p0 + p < a.np)
@@ -518,11 +685,17 @@ __global__ void __launch_bounds__(G_THREADS, 1)
         cluster_wait();
     }
     tc_fence_before();
-    __syncthreads();
+    if(PAIR > 1) // neither CTA leaves while the other's instructions or copies may reach it
+    {
+        cluster_arrive();
+        cluster_wait();
+    }
+    else
+        __syncthreads();
     if(warp == G_MMA_WARP)
     {
         tc_fence_after();
-        tmem_dealloc(tmem_base, G_TMEM_COLS);
+        tmem_dealloc<PAIR>(tmem_base, G_TMEM_COLS);
     }
 }
 
@@ -559,6 +732,21 @@ bool encode_codes(CUtensorMap* map, const void* codes, size_t rows, size_t pitch
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// scale tiles as (512 bytes, tile along k, band); box = the tiles of a stage x `bands`
+bool encode_scales(CUtensorMap* map, const void* scales, size_t tiles, size_t bands, int box_tiles, int box_bands)
+{
+    EncodeFn fn = encoder();
+    if(!fn)
+        return false;
+    const cuuint64_t dims[3]    = {MX4_TILE_BYTES / 4, (cuuint64_t)tiles, (cuuint64_t)bands};
+    const cuuint64_t strides[2] = {MX4_TILE_BYTES, (cuuint64_t)tiles * MX4_TILE_BYTES};
+    const cuuint32_t box[3]     = {MX4_TILE_BYTES / 4, (cuuint32_t)box_tiles, (cuuint32_t)box_bands};
+    const cuuint32_t estr[3]    = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(scales), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 constexpr int MAX_DEVICES = 64;
 
 // SMs of the current device; also binds the device's context to this thread, which the driver's encoder needs
@@ -592,49 +780,63 @@ struct Operand
 {
     const void* codes;
     const void* scales;
-    size_t      rows; // of the whole array: all groups
+    size_t      rows, bands; // of the whole array: all groups
 };
 
-template<int FMT, int BN>
-int launch(const GArgs& a, const Operand& p, const Operand& q, size_t pitch, int grid, cudaStream_t stream)
+template<int FMT, int BN, int PAIR>
+int launch(GArgs a, const Operand& p, const Operand& q, int sms, cudaStream_t stream)
 {
-    auto kernel = mx4_gemm_kernel<FMT, BN>;
-    using L     = GLayout<BN>;
-    CUtensorMap mp, mq;
-    if(!encode_codes(&mp, p.codes, p.rows, pitch, G_BP) || !encode_codes(&mq, q.codes, q.rows, pitch, BN))
+    using L      = GLayout<FMT, BN, PAIR>;
+    auto  kernel = mx4_gemm_kernel<FMT, BN, PAIR>;
+    const size_t pitch = mx4_pitch((size_t)a.K), k_tiles = mx4_tiles(FMT, (size_t)a.K);
+    Maps  maps;
+    if(!encode_codes(&maps.p, p.codes, p.rows, pitch, G_LANES) || !encode_codes(&maps.q, q.codes, q.rows, pitch, L::Q_ROWS)
+       || !encode_scales(&maps.scales_p, p.scales, k_tiles, p.bands, L::TILES, 1)
+       || !encode_scales(&maps.scales_q, q.scales, k_tiles, q.bands, L::TILES, L::Q_BANDS))
         return B200_SGEMM_NO_KERNEL;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM_BYTES);
+    a.tiles_p = (a.np + L::TILE_P - 1) / L::TILE_P;
+    // no more than these hold rows: groups start on multiples of 128, for wider tiles each can add one
+    unsigned long long tiles_q = ((unsigned long long)a.nq + BN - 1) / BN + (BN > MX4_BAND ? a.groups : 0);
+    const unsigned long long tiles = tiles_q * a.tiles_p;
+    if(tiles > 0x7fffffffull)
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    // one tile per cluster where K is split, otherwise as many CTAs as there are tiles or SMs
+    a.split = 1;
+    while(PAIR == 1 && a.groups == 0 && a.split < 8 && tiles * a.split * 2 <= (unsigned long long)sms && a.kblocks >= a.split * 4)
+        a.split *= 2;
+    const unsigned clusters = (unsigned)(a.split > 1 || tiles < (unsigned long long)(sms / PAIR) ? tiles : sms / PAIR);
+    cudaError_t    e        = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM_BYTES);
     if(e != cudaSuccess)
         return (int)e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3((unsigned)grid);
+    cfg.gridDim            = dim3(clusters * PAIR * a.split);
     cfg.blockDim           = dim3(G_THREADS);
     cfg.dynamicSmemBytes   = L::SMEM_BYTES;
     cfg.stream             = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id               = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.split;
+    attr[0].val.clusterDim.x = (unsigned)(PAIR * a.split);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs                = attr;
-    cfg.numAttrs             = a.split > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, a, mp, mq);
+    cfg.numAttrs             = PAIR * a.split > 1 ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, a, maps);
 }
 
 template<int FMT>
-int launch_tile(int bn, const GArgs& a, const Operand& p, const Operand& q, size_t pitch, int grid, cudaStream_t stream)
+int launch_tile(int bn, bool pair, const GArgs& a, const Operand& p, const Operand& q, int sms, cudaStream_t stream)
 {
+    if(pair)
+        return bn == 256 ? launch<FMT, 256, 2>(a, p, q, sms, stream) : launch<FMT, 128, 2>(a, p, q, sms, stream);
     if(bn == 32)
-        return launch<FMT, 32>(a, p, q, pitch, grid, stream);
+        return launch<FMT, 32, 1>(a, p, q, sms, stream);
     if(bn == 64)
-        return launch<FMT, 64>(a, p, q, pitch, grid, stream);
-    return launch<FMT, 128>(a, p, q, pitch, grid, stream);
+        return launch<FMT, 64, 1>(a, p, q, sms, stream);
+    return launch<FMT, 128, 1>(a, p, q, sms, stream);
 }
 
-// `a` holds what both entries agree on; `columns` is the expected number of rows of Q in a group, `tiles_q` the most column
-// tiles there can be for a tile width
-template<class TilesQ>
-int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_t columns, TilesQ tiles_q, cudaStream_t stream)
+// `a` holds what both entries agree on; `columns` is the expected number of rows of Q in a group
+int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_t columns, cudaStream_t stream)
 {
     int sms = 0, status = device_sms(&sms);
     if(status != B200_SGEMM_OK)
@@ -642,20 +844,19 @@ int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_
     a.K       = (int)K;
     a.kblocks = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
     a.chunk   = a.type == B200_SGEMM_F32 ? CHUNK_F32 : a.kblocks;
-    a.k_tiles = (int)mx4_tiles(format, K);
-    a.tiles_p = (a.np + G_BP - 1) / G_BP;
-    a.bands_p = a.tiles_p;
-    const int bn = columns <= 32 ? 32 : (columns <= 64 ? 64 : 128);
-    const unsigned long long tiles = (unsigned long long)a.tiles_p * tiles_q(bn);
-    if(tiles > 0x7fffffffull)
-        return B200_SGEMM_UNSUPPORTED_SIZE;
-    a.split = 1;
-    while(a.groups == 0 && a.split < 8 && tiles * a.split * 2 <= (unsigned long long)sms && a.kblocks >= a.split * 4)
-        a.split *= 2;
-    const int    grid  = a.split > 1 ? (int)tiles * a.split : (int)(tiles < (unsigned long long)sms ? tiles : sms);
-    const size_t pitch = mx4_pitch(K);
-    return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(bn, a, p, q, pitch, grid, stream)
-                                      : launch_tile<B200_SGEMM_MXFP4>(bn, a, p, q, pitch, grid, stream);
+    a.bands_p = (a.np + MX4_BAND - 1) / MX4_BAND;
+    int  bn   = columns <= 32 ? 32 : (columns <= 64 ? 64 : 128);
+    bool pair = false;
+    // pairs where they fill the SMs
+    const size_t groups = a.groups ? a.groups : 1;
+    const size_t pairs  = ((size_t)a.np + 255) / 256 * ((columns + 255) / 256) * groups;
+    if(columns > 128 && pairs >= (size_t)sms / 2)
+    {
+        pair = true;
+        bn   = a.type == B200_SGEMM_F32 ? 128 : 256;
+    }
+    return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(bn, pair, a, p, q, sms, stream)
+                                      : launch_tile<B200_SGEMM_MXFP4>(bn, pair, a, p, q, sms, stream);
 }
 } // namespace
 
@@ -678,7 +879,7 @@ extern "C" int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, con
         return B200_SGEMM_INVALID_ARGUMENT;
     if(ldc > (size_t(1) << 40))
         return B200_SGEMM_UNSUPPORTED_SIZE;
-    const Operand a{a_codes, a_scales, M}, b{b_codes, b_scales, N};
+    const Operand a{a_codes, a_scales, M, (M + MX4_BAND - 1) / MX4_BAND}, b{b_codes, b_scales, N, (N + MX4_BAND - 1) / MX4_BAND};
     // lanes: C's contiguous dimension, unless that one is short and the other is not
     bool b_lanes = row;
     if(packed <= 64 && (row ? M : N) > packed)
@@ -687,17 +888,13 @@ extern "C" int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, con
     g.c         = C;
     g.sp        = b_lanes == row ? 1 : (long long)ldc;
     g.sq        = b_lanes == row ? (long long)ldc : 1;
-    g.scales_p  = static_cast<const uint8_t*>(b_lanes ? b_scales : a_scales);
-    g.scales_q  = static_cast<const uint8_t*>(b_lanes ? a_scales : b_scales);
     g.global_p  = b_lanes ? global_b : global_a;
     g.global_q  = b_lanes ? global_a : global_b;
     g.alpha     = alpha;
     g.np        = (int)(b_lanes ? N : M);
     g.nq        = (int)(b_lanes ? M : N);
     g.type      = type_c;
-    const size_t nq = (size_t)g.nq;
-    return run(format, g, b_lanes ? b : a, b_lanes ? a : b, K, nq, [=](int bn) { return (nq + bn - 1) / bn; },
-               static_cast<cudaStream_t>(cuda_stream));
+    return run(format, g, b_lanes ? b : a, b_lanes ? a : b, K, (size_t)g.nq, static_cast<cudaStream_t>(cuda_stream));
 }
 
 extern "C" int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
@@ -722,8 +919,6 @@ extern "C" int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const voi
     g.c        = C;
     g.sp       = 1;
     g.sq       = (long long)ldc;
-    g.scales_p = static_cast<const uint8_t*>(b_scales);
-    g.scales_q = static_cast<const uint8_t*>(a_scales);
     g.offsets  = offsets;
     g.counts   = counts;
     g.global_p = global_b;
@@ -734,9 +929,9 @@ extern "C" int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const voi
     g.groups   = (int)groups;
     g.type     = type_c;
     const size_t used = used_rows && used_rows < rows ? used_rows : rows;
-    // groups start on multiples of 128 rows and so of any tile's width: no more tiles than these hold rows
-    return run(format, g, Operand{b_codes, b_scales, groups * N}, Operand{a_codes, a_scales, rows}, K, (used + groups - 1) / groups,
-               [=](int bn) { return (rows + bn - 1) / bn; }, static_cast<cudaStream_t>(cuda_stream));
+    const Operand b{b_codes, b_scales, groups * N, groups * ((N + MX4_BAND - 1) / MX4_BAND)};
+    const Operand a{a_codes, a_scales, rows, (rows + MX4_BAND - 1) / MX4_BAND};
+    return run(format, g, b, a, K, (used + groups - 1) / groups, static_cast<cudaStream_t>(cuda_stream));
 }
 
 extern "C" int b200_sgemm_mx4_device_status(int* status)

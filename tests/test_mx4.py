@@ -311,6 +311,24 @@ def test_product_many_tiles(sgemm, fmt, dtype):
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("layout_c", [0, 1])
+@pytest.mark.parametrize("shape", [(2100, 2300, 700), (2304, 2560, 64), (1025, 5000, 2049)], ids=lambda s: "x".join(map(str, s)))
+def test_product_by_pairs_of_ctas(sgemm, fmt, dtype, layout_c, shape):
+    M, N, K = shape
+    a, b = operand(fmt, M, K, 3), operand(fmt, N, K, 4)
+    n, m = (M, N) if layout_c == 0 else (N, M)
+    for ld in (m, m + 5):
+        c = torch.full((n, ld), 9.0, dtype=TYPES[dtype], device="cuda")
+        sgemm.gemm_mx4(fmt, layout_c, pkg.m_type[dtype], c, a[0], a[1], b[0], b[1], M, N, K, ldc=ld, alpha=0.5)
+        assert sgemm.mx4_device_status() == 0
+        assert (c[:, m:] == 9).all()
+        want = a[2] @ b[2].T * 0.5
+        check(c[:, :m] if layout_c == 0 else c[:, :m].T, want, ref.product_bound(a[2], b[2] * 0.5, want, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
 def test_product_exact_sums(sgemm, fmt):
     """Integers that the accumulator holds exactly come out exactly: one value per row and column, all of K."""
     M, N, K = 130, 140, 640
@@ -355,7 +373,7 @@ def grouped_case(fmt, counts, N, K, rows=None, seed=0):
 @pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("counts,N,K", [([1], 1, 1), ([3, 0, 130, 1], 200, 300), ([0, 0, 5], 128, 256), ([33, 64, 20, 0, 300], 130, 1000),
-                                        ([1] * 40, 300, 2048), ([0, 0], 64, 64), ([500, 700], 520, 512)],
+                                        ([1] * 40, 300, 2048), ([0, 0], 64, 64), ([500, 700], 520, 512), ([300, 0, 129, 700, 256, 1, 512, 400], 2200, 512)],
                          ids=lambda v: "-".join(map(str, v[:5])) if isinstance(v, list) else str(v))
 @pytest.mark.parametrize("hint", [0, 1])
 def test_grouped(sgemm, fmt, dtype, counts, N, K, hint):
