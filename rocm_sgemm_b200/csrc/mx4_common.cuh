@@ -55,12 +55,33 @@ struct Vec16
     __device__ __forceinline__ Vec16() {}
 };
 
-// e4m3 byte (0..0x7E) to its value
-__device__ __forceinline__ float e4m3_value(unsigned byte)
+// 32 bytes of T, in one access
+template<class T>
+struct Vec32
 {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
-    return __half2float(__half(h));
-}
+    static constexpr int N = 32 / sizeof(T);
+    union
+    {
+        uint32_t raw[8];
+        T        v[N];
+    };
+    __device__ __forceinline__ Vec32() {}
+    __device__ __forceinline__ void load(const T* p) // of read-only data
+    {
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7])
+                     : "l"(p));
+    }
+    __device__ __forceinline__ void store(T* p) const
+    {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(p), "r"(raw[0]), "r"(raw[1]), "r"(raw[2]), "r"(raw[3]), "r"(raw[4]), "r"(raw[5]), "r"(raw[6]), "r"(raw[7])
+                     : "memory");
+    }
+};
+
+// e4m3 byte (0..0x7E) to its value: its bits are those of an FP32 number 2^120 times smaller, subnormals included
+__device__ __forceinline__ float e4m3_value(unsigned byte) { return __uint_as_float(byte << 20) * 0x1p120f; }
 // value of an e8m0 byte below 0xFF: 2^(byte - 127)
 __device__ __forceinline__ float e8m0_value(unsigned byte) { return byte ? __uint_as_float(byte << 23) : __uint_as_float(1u << 22); }
 

@@ -50,7 +50,7 @@ constexpr int G_THREADS    = 320;
 constexpr int G_TMEM_COLS  = 512;
 constexpr int G_SCALE_COL  = 256; // tensor-memory columns 0..255: accumulators; behind them a slot of scales per stage
 constexpr int G_MAX_GROUPS = 1024;
-constexpr int CHUNK_F32    = 2; // K blocks (512 k, 8 products) added inside the tensor core for an FP32 result
+constexpr int CHUNK_F32    = 4; // K blocks (1024 k, 16 products) added inside the tensor core for an FP32 result
 
 constexpr int G_ERR_WAIT  = 1; // status bits: a wait gave up (bits 8.. say which);
 constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the matrix, the group was left out
@@ -188,7 +188,7 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, int rank)
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // what is in flight when a CTA gives up has to land before it leaves; bounded, without looking at the abort flag
 __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity)
@@ -598,28 +598,23 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                     if(!warp_wait(acc_full(buf), acc_ph, abort_flag)) { fail(3); ok = false; break; }
                     tc_fence_after();
                     const uint32_t from = tmem_base + buf * BN + half * COLS + (uint32_t(quarter * 32) << 16);
-                    constexpr int  STEP = COLS < 32 ? COLS : 32;
-    #pragma unroll
-                    for(int c = 0; c < COLS; c += STEP)
-                    {
-                        uint32_t v[STEP];
-    #pragma unroll
-                        for(int j = 0; j < STEP; j += 16)
-                            tmem_ld16(from + c + j, v + j);
-                        tmem_ld_wait();
-    #pragma unroll
-                        for(int j = 0; j < STEP; ++j)
-                            acc[c + j] = ch == 0 ? __uint_as_float(v[j]) : acc[c + j] + __uint_as_float(v[j]);
-                    }
+                    uint32_t v[COLS];
+#pragma unroll
+                    for(int j = 0; j < COLS; j += 16)
+                        tmem_ld16(from + j, v + j);
+                    tmem_ld_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if(lane == 0)
+                    if(lane == 0) // the accumulator is free before its values are added
                     {
                         if(PAIR > 1)
                             mbar_arrive_cluster(cluster_addr(acc_empty(buf), 0));
                         else
                             mbar_arrive(acc_empty(buf));
                     }
+#pragma unroll
+                    for(int j = 0; j < COLS; ++j)
+                        acc[j] = ch == 0 ? __uint_as_float(v[j]) : acc[j] + __uint_as_float(v[j]);
                     if(++buf == L::ACCS)
                     {
                         buf = 0;
@@ -637,7 +632,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                 else // park the part; a cluster has one tile, so the ring is at rest
                 {
                     float* part = reinterpret_cast<float*>(ring);
-    #pragma unroll
+#pragma unroll
                     for(int j = 0; j < COLS; ++j)
                         part[(q + j) * G_LANES + p] = acc[j];
                 }

@@ -14,9 +14,11 @@
 //   * the codes, g with at most 17 significant bits (1.0, powers of two): s g is exact in 21 bits, so every midpoint
 //     t s g is an FP32 number; the correctly rounded quotient (one product and two fused multiply-adds) is then on the
 //     same side of t as x / (s g), or on t when that is.
-//   * any other g: the quotient is a product with the reciprocal, off by three units at most.  Midpoints have two bits
-//     after the leading one; where a quotient comes within eight units of such a number (one in 10^5) the block is done
-//     again by the signs of |x| - (t s) g, exact as above.
+//   * any other g: products with the reciprocal, made a little too small and a little too large (2^-21, five roundings of
+//     2^-24 lie in between), bracket the quotient.  Where their codes differ the value is read again and the sign of
+//     |x| - (t s) g decides, exact as above.  That is rare for random g, but g = amax / 2688 of BF16 data makes every
+//     hundredth block hold such a value, so a warp meets one in most rows: the repair has to be cheap (doing all sixteen
+//     values again by comparisons took 271 us for 16384 x 8192 BF16 where g was of that kind, 151 us where not).
 #include "mx4_common.cuh"
 
 namespace
@@ -26,6 +28,9 @@ using namespace sgemm_b200;
 constexpr int Q_THREADS = 256;
 constexpr int Q_LANE_K  = 16;            // k of one lane: a block of nvfp4, half of one of mxfp4
 constexpr int Q_TILE_K  = 32 * Q_LANE_K; // k of one warp's step, and of one CTA
+constexpr int Q_WARP_ROWS = 4;           // rows of one warp
+constexpr int Q_ROWS      = Q_THREADS / 32 * Q_WARP_ROWS;
+static_assert(Q_ROWS == 32, "the rows of a CTA lie 16 bytes apart in a scale tile");
 constexpr int Q_COL_K   = 128;           // k of one CTA when the rows are the contiguous dimension
 
 constexpr unsigned INF_BITS  = 0x7F800000u;
@@ -59,32 +64,19 @@ __device__ __forceinline__ Scale scale_nvfp4(unsigned amax_bits, const Global& G
     Scale       r;
     const float amax = __uint_as_float(amax_bits);
     unsigned    c    = __nv_cvt_float_to_fp8(amax * G.r6, __NV_SATFINITE, __NV_E4M3);
-    float       v    = e4m3_value(c);
-    if(c < 0x7Eu)
-    {
-        const float up = e4m3_value(c + 1);
-        const float d  = fmaf(-3.f * (v + up), G.g, amax); // amax - 6 * (v + up) / 2 * g
-        if(d > 0.f || (d == 0.f && (c & 1u)))
-        {
-            ++c;
-            v = up;
-        }
-    }
-    if(c > 0u)
-    {
-        const float dn = e4m3_value(c - 1);
-        const float d  = fmaf(-3.f * (v + dn), G.g, amax);
-        if(d < 0.f || (d == 0.f && (c & 1u)))
-        {
-            --c;
-            v = dn;
-        }
-    }
+    // amax - 6 m g for the midpoints m above and below c (half a step on in the bits)
+    const float above = fmaf(-(__uint_as_float((2 * c + 1) << 19) * (6.f * 0x1p120f)), G.g, amax);
+    const float below = fmaf(-(__uint_as_float((2 * c - 1) << 19) * (6.f * 0x1p120f)), G.g, amax);
+    if(c < 0x7Eu && (above > 0.f || (above == 0.f && (c & 1u))))
+        ++c;
+    else if(c > 0u && (below < 0.f || (below == 0.f && (c & 1u))))
+        --c;
     const bool bad = amax_bits >= INF_BITS || !G.ok;
     r.byte = bad ? NAN_E4M3 : c;
-    r.s    = v;
-    r.sg   = v * G.g;
-    r.inv  = bad || c == 0u ? 0.f : __frcp_rn(r.sg);
+    r.s    = e4m3_value(c);
+    r.sg   = r.s * G.g;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv) : "f"(r.sg)); // within 2^-23; s g is in 2^+-100
+    r.inv = bad || c == 0u ? 0.f : r.inv;
     return r;
 }
 __device__ __forceinline__ Scale scale_mxfp4(unsigned amax_bits)
@@ -98,83 +90,92 @@ __device__ __forceinline__ Scale scale_mxfp4(unsigned amax_bits)
     return r;
 }
 
-// code of one value by exact comparison with the midpoints
-__device__ __noinline__ unsigned code_exact(float x, float s, float g)
+// what a code 0..7 stands for
+__device__ __forceinline__ float e2m1_value(unsigned code) { return __uint_as_float(code << 22) * 0x1p126f; }
+
+// the codes nearest to y[0..15], eight bytes
+__device__ __forceinline__ uint2 codes16(const float2 (&y)[Q_LANE_K / 2])
 {
-    const float a    = fabsf(x);
-    unsigned    code = 0;
-    const float mid[7] = {0.25f, 0.75f, 1.25f, 1.75f, 2.5f, 3.5f, 5.f};
+    uint2 out = make_uint2(0u, 0u);
 #pragma unroll
-    for(int i = 0; i < 7; ++i)
+    for(int i = 0; i < 4; ++i)
     {
-        const float d = fmaf(-(mid[i] * s), g, a);
-        code += d > 0.f || (d == 0.f && (i & 1)) ? 1u : 0u;
+        out.x |= (unsigned)__nv_cvt_float2_to_fp4x2(y[i], __NV_E2M1, cudaRoundNearest) << (8 * i);
+        out.y |= (unsigned)__nv_cvt_float2_to_fp4x2(y[4 + i], __NV_E2M1, cudaRoundNearest) << (8 * i);
     }
-    return code | (__float_as_uint(x) >> 31 << 3);
+    return out;
+}
+// y = x * f, two values an instruction
+__device__ __forceinline__ void scaled16(float2 (&y)[Q_LANE_K / 2], const float (&x)[Q_LANE_K], float f)
+{
+#pragma unroll
+    for(int i = 0; i < Q_LANE_K / 2; ++i)
+        y[i] = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(f, f));
+}
+
+// the values behind the nibbles in which `low` and `high` differ, by exact comparison; again(i) is x[i]
+template<class Again>
+__device__ __forceinline__ unsigned settle(unsigned low, unsigned high, int first, const Scale& sc, const Global& G, Again again)
+{
+    for(unsigned left = low ^ high; left;)
+    {
+        const int      i    = (__ffs(left) - 1) >> 2;
+        const unsigned code = low >> (4 * i) & 7u; // and code + 1 is the other one
+        const float    mid  = 0.5f * (e2m1_value(code) + e2m1_value(code + 1));
+        const float    d    = fmaf(-(mid * sc.s), G.g, fabsf(again(first + i)));
+        if(d > 0.f || (d == 0.f && (code & 1u)))
+            low += 1u << (4 * i);
+        left &= ~(0xFu << (4 * i));
+    }
+    return low;
 }
 
 // sixteen codes, eight bytes
-template<int FMT>
-__device__ __forceinline__ uint2 encode(const float (&x)[Q_LANE_K], const Scale& sc, const Global& G)
+template<int FMT, class Again>
+__device__ __forceinline__ uint2 encode(const float (&x)[Q_LANE_K], const Scale& sc, const Global& G, Again again)
 {
-    uint2 out = make_uint2(0u, 0u);
     if(sc.inv == 0.f)
-        return out;
-    float y[Q_LANE_K];
-    bool  near = false;
+        return make_uint2(0u, 0u);
+    float2 y[Q_LANE_K / 2];
     if(FMT == B200_SGEMM_MXFP4)
     {
-#pragma unroll
-        for(int i = 0; i < Q_LANE_K; ++i)
-            y[i] = x[i] * sc.inv;
+        scaled16(y, x, sc.inv);
+        return codes16(y);
     }
-    else if(G.few)
+    if(G.few)
     {
 #pragma unroll
         for(int i = 0; i < Q_LANE_K; ++i)
         {
             const float q = x[i] * sc.inv;
-            y[i]          = copysignf(fmaf(fmaf(-q, sc.sg, x[i]), sc.inv, q), x[i]); // -0 keeps its sign
-        }
-    }
-    else
-    {
-#pragma unroll
-        for(int i = 0; i < Q_LANE_K; ++i)
-        {
-            y[i] = x[i] * sc.inv;
-            near = near || ((__float_as_uint(y[i]) + 8u) & 0x1FFFFFu) <= 16u;
-        }
-    }
-    if(near)
-    {
-#pragma unroll
-        for(int i = 0; i < Q_LANE_K; ++i)
-        {
-            const unsigned c = code_exact(x[i], sc.s, G.g);
-            if(i < 8)
-                out.x |= c << (4 * i);
+            const float v = copysignf(fmaf(fmaf(-q, sc.sg, x[i]), sc.inv, q), x[i]); // -0 keeps its sign
+            if(i & 1)
+                y[i / 2].y = v;
             else
-                out.y |= c << (4 * (i - 8));
+                y[i / 2].x = v;
         }
-        return out;
+        return codes16(y);
     }
-#pragma unroll
-    for(int i = 0; i < 4; ++i)
+    scaled16(y, x, sc.inv * (1.f - 0x1p-21f));
+    uint2 low = codes16(y);
+    scaled16(y, x, sc.inv * (1.f + 0x1p-21f));
+    const uint2 high = codes16(y);
+    if(low.x != high.x || low.y != high.y)
     {
-        out.x |= (unsigned)__nv_cvt_float2_to_fp4x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_E2M1, cudaRoundNearest) << (8 * i);
-        out.y |= (unsigned)__nv_cvt_float2_to_fp4x2(make_float2(y[8 + 2 * i], y[9 + 2 * i]), __NV_E2M1, cudaRoundNearest) << (8 * i);
+        low.x = settle(low.x, high.x, 0, sc, G, again);
+        low.y = settle(low.y, high.y, 8, sc, G, again);
     }
-    return out;
+    return low;
 }
 
+// largest magnitude as bits; NaN where there is one
 __device__ __forceinline__ unsigned amax16(const float (&x)[Q_LANE_K])
 {
-    unsigned m = 0;
+    float m = 0.f;
 #pragma unroll
-    for(int i = 0; i < Q_LANE_K; ++i)
-        m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu); // NaN orders above infinity
-    return m;
+    for(int i = 0; i < Q_LANE_K; i += 2)
+        asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(x[i])), "f"(fabsf(x[i + 1])));
+    return __float_as_uint(m);
 }
 
 struct QArgs
@@ -186,100 +187,102 @@ struct QArgs
     uint8_t*     scales;
     long long    ld, pitch;
     int          rows, source_rows, K, tiles, index_div;
-    int          vector; // base and pitch of X allow 16-byte loads
+    int          vector; // base and pitch of X allow 32-byte loads
 };
 
-// position of (row in band, block in CTA) in the staged scale tiles; the pad keeps tiles in different banks
-constexpr int Q_TILE_PAD = MX4_TILE_BYTES + 16;
-__device__ __forceinline__ int scale_at(int row, int block)
+// address of (row, block) in the scales
+__device__ __forceinline__ size_t scale_at(long long row, int block, int tiles)
 {
-    return (block >> 2) * Q_TILE_PAD + (row & 31) * 16 + (row >> 5) * 4 + (block & 3);
-}
-// staged tiles to their place; the band's tiles from `first` on
-__device__ __forceinline__ void store_scales(const uint8_t* staged, const QArgs& a, int band, int first, int count)
-{
-    count = min(count, a.tiles - first);
-    uint4* dst = reinterpret_cast<uint4*>(a.scales + ((size_t)band * a.tiles + first) * MX4_TILE_BYTES);
-    for(int i = threadIdx.x; i < count * (MX4_TILE_BYTES / 16); i += Q_THREADS)
-        dst[i] = *reinterpret_cast<const uint4*>(staged + (i >> 5) * Q_TILE_PAD + (i & 31) * 16);
+    return ((size_t)(row / MX4_BAND) * tiles + (block >> 2)) * MX4_TILE_BYTES + (row & 31) * 16 + ((row & (MX4_BAND - 1)) >> 5) * 4
+           + (block & 3);
 }
 
-// K-contiguous source.  One CTA: a band of 128 rows x 512 k; a warp takes a row at a time, a lane 16 neighbours of it,
-// so a row is read and written in contiguous pieces of a warp's width.  The scales of the band meet in shared memory
-// and leave as whole tiles.
+// K-contiguous source.  One CTA: 32 rows (a quarter of a band) x 512 k.  A warp takes four rows, the next fetched while one is
+// worked on, a lane 16 neighbours of each in one or two 32-byte loads; codes leave in contiguous pieces of a warp's width.  Scales meet in shared
+// memory and leave as words of four blocks.  (With a whole band per CTA, 16 rows per warp one after the other, 16384 x 8192
+// BF16 took 163 us and 4097 x 2050 had only 165 CTAs.)
 template<int FMT, class T>
 __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_constant__ QArgs a)
 {
     constexpr int BLOCKS = Q_TILE_K / (FMT == B200_SGEMM_NVFP4 ? 16 : 32), TILES = BLOCKS / 4;
-    __shared__ __align__(16) uint8_t staged[TILES * Q_TILE_PAD];
-    __shared__ int any;
-    const int  k_ctas = (a.K + Q_TILE_K - 1) / Q_TILE_K;
-    const int  band = blockIdx.x / k_ctas, kc = blockIdx.x % k_ctas;
-    const int  warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int  k0 = kc * Q_TILE_K + lane * Q_LANE_K;
-    const T*   X  = static_cast<const T*>(a.x);
-    if(a.row_index) // a band of the sorted rows that holds none is left alone
+    __shared__ __align__(16) uint8_t staged[Q_ROWS][BLOCKS];
+    const int       k_ctas = (a.K + Q_TILE_K - 1) / Q_TILE_K;
+    const int       slice = blockIdx.x / k_ctas, kc = blockIdx.x - slice * k_ctas;
+    const long long row0 = (long long)slice * Q_ROWS;
+    const int       warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int       k0 = kc * Q_TILE_K + lane * Q_LANE_K;
+    const T*        X  = static_cast<const T*>(a.x);
+    if(a.row_index) // a band of the gathered rows that holds none is left alone
     {
-        if(threadIdx.x == 0)
-            any = 0;
-        __syncthreads();
-        const int r = band * MX4_BAND + threadIdx.x;
-        if(threadIdx.x < MX4_BAND && r < a.rows && a.row_index[r] >= 0)
-            any = 1;
-        __syncthreads();
-        if(!any)
+        const long long r = row0 / MX4_BAND * MX4_BAND + threadIdx.x;
+        const int       index = threadIdx.x < MX4_BAND && r < a.rows ? __ldg(a.row_index + r) : -1;
+        if(!__syncthreads_or(index >= 0 && index / a.index_div < a.source_rows))
             return;
     }
+    const bool vector = a.vector && k0 + Q_LANE_K <= a.K;
+    // the row of X behind row r of the slice, uniform over the warp; -1: none
+    auto source = [&](int r) -> long long {
+        const long long row = row0 + r;
+        if(row >= a.rows)
+            return -1;
+        if(!a.row_index)
+            return row;
+        const int index = __ldg(a.row_index + row), src = index < 0 ? -1 : index / a.index_div;
+        return src < a.source_rows ? src : -1;
+    };
+    constexpr int V = Q_LANE_K / Vec32<T>::N;
+    Vec32<T>      ahead[V]; // a row is fetched while the one before is worked on
+    auto fetch = [&](long long src) {
+        if(vector && src >= 0)
+        {
+#pragma unroll
+            for(int j = 0; j < V; ++j)
+                ahead[j].load(X + src * a.ld + k0 + j * Vec32<T>::N);
+        }
+    };
+    long long next = source(warp);
+    fetch(next);
     const Global G = load_global(a.global);
-    for(int i = threadIdx.x; i < TILES * Q_TILE_PAD / 16; i += Q_THREADS)
-        reinterpret_cast<uint4*>(staged)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    const int in_band = min(MX4_BAND, a.rows - band * MX4_BAND);
-#pragma unroll 2
-    for(int r = warp; r < in_band; r += Q_THREADS / 32)
+#pragma unroll 1
+    for(int r = warp; r < Q_ROWS; r += Q_THREADS / 32)
     {
-        const long long row = (long long)band * MX4_BAND + r;
-        long long       src = row;
-        if(a.row_index)
-        {
-            const int index = a.row_index[row];
-            src             = index < 0 ? -1 : index / a.index_div;
-            if(src < 0 || src >= a.source_rows)
-                continue; // uniform over the warp
-        }
-        const T* from = X + src * a.ld + k0;
-        float    x[Q_LANE_K];
-        if(a.vector && k0 + Q_LANE_K <= a.K)
-        {
-            constexpr int N = Vec16<T>::N;
-            Vec16<T>      v[Q_LANE_K / N];
+        const long long src = next;
+        float           x[Q_LANE_K];
 #pragma unroll
-            for(int i = 0; i < Q_LANE_K / N; ++i)
-                v[i].raw = __ldg(reinterpret_cast<const uint4*>(from) + i);
-#pragma unroll
-            for(int i = 0; i < Q_LANE_K; ++i)
-                x[i] = to_float(v[i / N].v[i % N]);
-        }
-        else
+        for(int j = 0; j < Q_LANE_K; ++j)
         {
-#pragma unroll
-            for(int i = 0; i < Q_LANE_K; ++i)
-                x[i] = k0 + i < a.K ? to_float(from[i]) : 0.f;
+            if(vector)
+                x[j] = to_float(ahead[j / Vec32<T>::N].v[j % Vec32<T>::N]);
+            else
+                x[j] = src >= 0 && k0 + j < a.K ? to_float(X[src * a.ld + k0 + j]) : 0.f;
         }
-        unsigned amax = amax16(x);
-        if(FMT == B200_SGEMM_MXFP4)
-            amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-        const Scale sc = FMT == B200_SGEMM_NVFP4 ? scale_nvfp4(amax, G) : scale_mxfp4(amax);
-        const uint2 c  = encode<FMT>(x, sc, G);
-        if(k0 < 2 * a.pitch)
-            *reinterpret_cast<uint2*>(a.codes + row * a.pitch + k0 / 2) = c;
+        next = r + Q_THREADS / 32 < Q_ROWS ? source(r + Q_THREADS / 32) : -1;
+        fetch(next);
+        Scale sc;
+        sc.byte = 0;
+        if(src >= 0)
+        {
+            unsigned amax = amax16(x);
+            if(FMT == B200_SGEMM_MXFP4)
+                amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1)); // NaN orders above infinity
+            sc            = FMT == B200_SGEMM_NVFP4 ? scale_nvfp4(amax, G) : scale_mxfp4(amax);
+            const uint2 c = encode<FMT>(x, sc, G, [&](int i) { return to_float(X[src * a.ld + k0 + i]); });
+            if(k0 < 2 * a.pitch)
+                *reinterpret_cast<uint2*>(a.codes + (row0 + r) * a.pitch + k0 / 2) = c;
+        }
         if(FMT == B200_SGEMM_NVFP4)
-            staged[scale_at(r, lane)] = (uint8_t)sc.byte;
+            staged[r][lane] = (uint8_t)sc.byte;
         else if((lane & 1) == 0)
-            staged[scale_at(r, lane >> 1)] = (uint8_t)sc.byte;
+            staged[r][lane >> 1] = (uint8_t)sc.byte;
     }
     __syncthreads();
-    store_scales(staged, a, band, kc * TILES, TILES);
+    for(int i = threadIdx.x; i < Q_ROWS * TILES; i += Q_THREADS)
+    {
+        const int tile = i / Q_ROWS, r = i % Q_ROWS;
+        if(kc * TILES + tile < a.tiles)
+            *reinterpret_cast<uint32_t*>(a.scales + scale_at(row0 + r, (kc * TILES + tile) * 4, a.tiles)) =
+                *reinterpret_cast<const uint32_t*>(&staged[r][tile * 4]);
+    }
 }
 
 // Row-contiguous source (a col-major A, a row-major B).  One CTA: a band of 128 rows x 128 k; a thread takes one row and
@@ -288,15 +291,15 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_c
 template<int FMT, class T>
 __global__ void __launch_bounds__(Q_THREADS) quantize_cols_kernel(const __grid_constant__ QArgs a)
 {
-    constexpr int BLOCKS = Q_COL_K / (FMT == B200_SGEMM_NVFP4 ? 16 : 32), TILES = BLOCKS / 4;
-    __shared__ __align__(16) uint8_t staged[TILES * Q_TILE_PAD];
+    constexpr int   BLOCK = FMT == B200_SGEMM_NVFP4 ? 16 : 32;
     const int       k_ctas = (a.K + Q_COL_K - 1) / Q_COL_K;
-    const int       band = blockIdx.x / k_ctas, kc = blockIdx.x % k_ctas;
+    const int       band = blockIdx.x / k_ctas, kc = blockIdx.x - band * k_ctas;
     const int       r = threadIdx.x & (MX4_BAND - 1), half = threadIdx.x / MX4_BAND;
     const long long row = (long long)band * MX4_BAND + r;
     const T*        X   = static_cast<const T*>(a.x);
     const Global    G   = load_global(a.global);
     const bool      in  = row < a.rows;
+    unsigned        word = 0; // the scales of the thread's 64 k
 #pragma unroll
     for(int j = 0; j < 2; ++j) // 32 k at a time
     {
@@ -314,16 +317,25 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_cols_kernel(const __grid_c
             sc[0] = scale_nvfp4(amax[0], G);
             sc[1] = scale_nvfp4(amax[1], G);
         }
-        const uint2 lo = encode<FMT>(x[0], sc[0], G), hi = encode<FMT>(x[1], sc[1], G);
+        auto        again = [&](int i) { return to_float(X[(long long)(k0 + i) * a.ld + row]); };
+        const uint2 lo = encode<FMT>(x[0], sc[0], G, again);
+        const uint2 hi = encode<FMT>(x[1], sc[1], G, [&](int i) { return again(16 + i); });
         if(in && k0 < 2 * a.pitch)
             *reinterpret_cast<uint4*>(a.codes + row * a.pitch + k0 / 2) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        const int block = (half * 64 + j * 32) / (FMT == B200_SGEMM_NVFP4 ? 16 : 32);
-        staged[scale_at(r, block)] = in ? (uint8_t)sc[0].byte : 0;
         if(FMT == B200_SGEMM_NVFP4)
-            staged[scale_at(r, block + 1)] = in ? (uint8_t)sc[1].byte : 0;
+            word |= (sc[0].byte | sc[1].byte << 8) << (16 * j);
+        else
+            word |= sc[0].byte << (8 * j);
     }
-    __syncthreads();
-    store_scales(staged, a, band, kc * TILES, TILES);
+    const int block = (kc * Q_COL_K + half * 64) / BLOCK;
+    if(block >> 2 < a.tiles)
+    {
+        uint8_t* to = a.scales + scale_at(row, block, a.tiles);
+        if(FMT == B200_SGEMM_NVFP4)
+            *reinterpret_cast<uint32_t*>(to) = in ? word : 0u;
+        else
+            *reinterpret_cast<uint16_t*>(to) = in ? (uint16_t)word : (uint16_t)0;
+    }
 }
 
 struct DArgs
@@ -334,75 +346,131 @@ struct DArgs
     void*          x;
     long long      ld, pitch;
     int            rows, K, tiles;
-    int            vector;
 };
 
-// One CTA: a band of 128 rows x 512 k.  The scale tiles come in whole; a lane turns 16 bytes of output at a time, so that
-// a warp's stores are contiguous.
+// the two values of a byte of codes
+__device__ __forceinline__ float2 levels2(unsigned byte)
+{
+    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1);
+    return __half22float2(__half2(h));
+}
+// the value of a scale byte
+template<int FMT>
+__device__ __forceinline__ float scale_value(unsigned byte)
+{
+    const float nan = __uint_as_float(0x7FC00000u);
+    if(FMT == B200_SGEMM_NVFP4)
+        return (byte & 0x7Fu) == NAN_E4M3 ? nan : e4m3_value(byte);
+    return byte == NAN_E8M0 ? nan : e8m0_value(byte);
+}
+
+// One CTA: 32 rows x 512 k, a warp four rows.  A lane turns 32 bytes of output at a time, with the codes and scales of all four
+// rows in flight at once.
 template<int FMT, class T>
 __global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const __grid_constant__ DArgs a)
 {
-    constexpr int BLOCK = FMT == B200_SGEMM_NVFP4 ? 16 : 32, TILES = Q_TILE_K / BLOCK / 4;
-    constexpr int N = Vec16<T>::N;
-    __shared__ __align__(16) uint8_t staged[TILES * Q_TILE_PAD];
-    const int k_ctas = (a.K + Q_TILE_K - 1) / Q_TILE_K;
-    const int band = blockIdx.x / k_ctas, kc = blockIdx.x % k_ctas;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    {
-        const int    count = min(TILES, a.tiles - kc * TILES);
-        const uint4* src = reinterpret_cast<const uint4*>(a.scales + ((size_t)band * a.tiles + kc * TILES) * MX4_TILE_BYTES);
-        for(int i = threadIdx.x; i < count * (MX4_TILE_BYTES / 16); i += Q_THREADS)
-            *reinterpret_cast<uint4*>(staged + (i >> 5) * Q_TILE_PAD + (i & 31) * 16) = __ldg(src + i);
-    }
-    const float g = a.global ? *a.global : 1.f;
-    __syncthreads();
-    const int in_band = min(MX4_BAND, a.rows - band * MX4_BAND);
-    for(int r = warp; r < in_band; r += Q_THREADS / 32)
-    {
-        const long long row = (long long)band * MX4_BAND + r;
+    constexpr int   BLOCK = FMT == B200_SGEMM_NVFP4 ? 16 : 32, N = Vec32<T>::N, STEPS = Q_TILE_K / (32 * N);
+    const int       k_ctas = (a.K + Q_TILE_K - 1) / Q_TILE_K;
+    const int       slice = blockIdx.x / k_ctas, kc = blockIdx.x - slice * k_ctas;
+    const int       warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long row0 = (long long)slice * Q_ROWS + warp;
+    const float     g = a.global ? *a.global : 1.f;
+    uint2           c[Q_WARP_ROWS][STEPS];
+    uint8_t         byte[Q_WARP_ROWS][STEPS];
 #pragma unroll
-        for(int step = 0; step < Q_TILE_K / (32 * N); ++step)
+    for(int i = 0; i < Q_WARP_ROWS; ++i)
+    {
+        const long long row = row0 + i * (Q_THREADS / 32);
+#pragma unroll
+        for(int step = 0; step < STEPS; ++step)
         {
-            const int kl = step * 32 * N + lane * N, k0 = kc * Q_TILE_K + kl;
-            if(k0 >= a.K)
-                break;
-            const uint8_t* from = a.codes + row * a.pitch + k0 / 2;
-            unsigned       c;
-            if(N == 8)
-                c = __ldg(reinterpret_cast<const unsigned*>(from));
-            else
-                c = __ldg(reinterpret_cast<const unsigned short*>(from));
-            const unsigned byte = staged[scale_at(r, kl / BLOCK)];
-            const float    s    = FMT == B200_SGEMM_NVFP4
-                                      ? ((byte & 0x7Fu) == NAN_E4M3 ? __uint_as_float(0x7FC00000u) : e4m3_value(byte))
-                                      : (byte == NAN_E8M0 ? __uint_as_float(0x7FC00000u) : e8m0_value(byte));
-            Vec16<T> out;
-#pragma unroll
-            for(int i = 0; i < N / 2; ++i)
+            const int k = kc * Q_TILE_K + (step * 32 + lane) * N;
+            if(row < a.rows && k < a.K)
             {
-                const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(c >> (8 * i) & 0xFFu), __NV_E2M1);
-                const float2      f = __half22float2(__half2(h));
-                out.v[2 * i]     = from_float<T>(f.x * s * g); // f * s is exact
-                out.v[2 * i + 1] = from_float<T>(f.y * s * g);
+                const uint8_t* from = a.codes + row * a.pitch + k / 2;
+                if(N == 16)
+                    c[i][step] = __ldg(reinterpret_cast<const uint2*>(from));
+                else
+                    c[i][step].x = __ldg(reinterpret_cast<const unsigned*>(from));
+                byte[i][step] = __ldg(a.scales + scale_at(row, k / BLOCK, a.tiles));
             }
-            T* to = static_cast<T*>(a.x) + row * a.ld + k0;
-            if(a.vector && k0 + N <= a.K)
-                *reinterpret_cast<uint4*>(to) = out.raw;
+        }
+    }
+#pragma unroll
+    for(int i = 0; i < Q_WARP_ROWS; ++i)
+    {
+        const long long row = row0 + i * (Q_THREADS / 32);
+#pragma unroll
+        for(int step = 0; step < STEPS; ++step)
+        {
+            const int k = kc * Q_TILE_K + (step * 32 + lane) * N;
+            if(row >= a.rows || k >= a.K)
+                break;
+            const float s  = scale_value<FMT>(byte[i][step]);
+            T*          to = static_cast<T*>(a.x) + row * a.ld + k;
+            Vec32<T>    out;
+#pragma unroll
+            for(int j = 0; j < N / 2; ++j)
+            {
+                const float2 f = levels2((j < 4 ? c[i][step].x >> (8 * j) : c[i][step].y >> (8 * (j - 4))) & 0xFFu);
+                out.v[2 * j]     = from_float<T>(f.x * s * g); // f * s is exact
+                out.v[2 * j + 1] = from_float<T>(f.y * s * g);
+            }
+            if(k + N <= a.K)
+                out.store(to);
             else
             {
 #pragma unroll
-                for(int i = 0; i < N; ++i)
-                    if(k0 + i < a.K)
-                        to[i] = out.v[i];
+                for(int j = 0; j < N; ++j)
+                    if(k + j < a.K)
+                        to[j] = out.v[j];
             }
         }
     }
 }
 
-// CTAs of bands x pieces of k, or 0 when that is more than a grid holds
-unsigned grid_of(size_t rows, size_t K, size_t tile_k)
+// The same for rows that do not start on 32 bytes: lanes take neighbours, so that a warp's stores are contiguous all the same.
+// Each lane turns one scale of the row into its value and the others fetch it from there.
+template<int FMT, class T>
+__global__ void __launch_bounds__(Q_THREADS) dequantize_unaligned_kernel(const __grid_constant__ DArgs a)
 {
-    const unsigned long long n = (unsigned long long)((rows + MX4_BAND - 1) / MX4_BAND) * ((K + tile_k - 1) / tile_k);
+    constexpr int   BLOCK = FMT == B200_SGEMM_NVFP4 ? 16 : 32, STEPS = Q_TILE_K / 32;
+    const int       k_ctas = (a.K + Q_TILE_K - 1) / Q_TILE_K;
+    const int       slice = blockIdx.x / k_ctas, kc = blockIdx.x - slice * k_ctas;
+    const int       warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float     g = a.global ? *a.global : 1.f;
+    const int       k0 = kc * Q_TILE_K + lane, block = kc * (Q_TILE_K / BLOCK) + lane % (Q_TILE_K / BLOCK);
+#pragma unroll 2
+    for(int i = 0; i < Q_WARP_ROWS; ++i)
+    {
+        const long long row = (long long)slice * Q_ROWS + warp + i * (Q_THREADS / 32);
+        if(row >= a.rows)
+            break;
+        const uint8_t* from = a.codes + row * a.pitch + k0 / 2;
+        uint8_t        c[STEPS];
+#pragma unroll
+        for(int step = 0; step < STEPS; ++step)
+            if(k0 + step * 32 < a.K)
+                c[step] = __ldg(from + step * 16);
+        const float value = scale_value<FMT>(block >> 2 < a.tiles ? __ldg(a.scales + scale_at(row, block, a.tiles)) : 0);
+        T*          to    = static_cast<T*>(a.x) + row * a.ld + k0;
+#pragma unroll
+        for(int step = 0; step < STEPS; ++step)
+        {
+            const float s = __shfl_sync(0xFFFFFFFFu, value, (step * 32 + lane) / BLOCK);
+            if(k0 + step * 32 < a.K)
+            {
+                const float2 f = levels2(c[step]);
+                to[step * 32]  = from_float<T>((lane & 1 ? f.y : f.x) * s * g);
+            }
+        }
+    }
+}
+
+// CTAs of `parts` x pieces of k, or 0 when that is more than a grid holds
+unsigned grid_of(size_t parts, size_t K, size_t tile_k)
+{
+    const unsigned long long n = (unsigned long long)parts * ((K + tile_k - 1) / tile_k);
     return n > 0x7fffffffull ? 0u : (unsigned)n;
 }
 } // namespace
@@ -436,7 +504,8 @@ extern "C" int b200_sgemm_mx4_quantize(int format, int layout, int type, const v
     if(ldx < extent || misaligned(X, type_bytes(type)) || misaligned(codes, 16) || misaligned(scales, 16)
        || misaligned(row_index, 4) || misaligned(global_scale, 4) || (format == B200_SGEMM_MXFP4 && global_scale))
         return B200_SGEMM_INVALID_ARGUMENT;
-    const unsigned grid = grid_of(rows, K, row_major ? Q_TILE_K : Q_COL_K);
+    const size_t   bands = (rows + MX4_BAND - 1) / MX4_BAND;
+    const unsigned grid  = row_major ? grid_of(bands * (MX4_BAND / Q_ROWS), K, Q_TILE_K) : grid_of(bands, K, Q_COL_K);
     if(!grid || ldx > (size_t(1) << 40))
         return B200_SGEMM_UNSUPPORTED_SIZE;
     QArgs a;
@@ -452,7 +521,7 @@ extern "C" int b200_sgemm_mx4_quantize(int format, int layout, int type, const v
     a.K           = (int)K;
     a.tiles       = (int)mx4_tiles(format, K);
     a.index_div   = index_div;
-    a.vector      = !misaligned(X, 16) && ldx * type_bytes(type) % 16 == 0;
+    a.vector      = !misaligned(X, 32) && ldx * type_bytes(type) % 32 == 0;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
@@ -486,7 +555,7 @@ extern "C" int b200_sgemm_mx4_dequantize(int format, int type, const void* codes
     if(ldx < K || misaligned(X, type_bytes(type)) || misaligned(codes, 16) || misaligned(scales, 16)
        || misaligned(global_scale, 4) || (format == B200_SGEMM_MXFP4 && global_scale))
         return B200_SGEMM_INVALID_ARGUMENT;
-    const unsigned grid = grid_of(rows, K, Q_TILE_K);
+    const unsigned grid = grid_of((rows + Q_ROWS - 1) / Q_ROWS, K, Q_TILE_K);
     if(!grid || ldx > (size_t(1) << 40))
         return B200_SGEMM_UNSUPPORTED_SIZE;
     DArgs a;
@@ -499,14 +568,14 @@ extern "C" int b200_sgemm_mx4_dequantize(int format, int type, const void* codes
     a.rows   = (int)rows;
     a.K      = (int)K;
     a.tiles  = (int)mx4_tiles(format, K);
-    a.vector = !misaligned(X, 16) && ldx * type_bytes(type) % 16 == 0;
+    const bool vector = !misaligned(X, 32) && ldx * type_bytes(type) % 32 == 0;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        if(format == B200_SGEMM_NVFP4)
-            dequantize_kernel<B200_SGEMM_NVFP4, T><<<grid, Q_THREADS, 0, stream>>>(a);
-        else
-            dequantize_kernel<B200_SGEMM_MXFP4, T><<<grid, Q_THREADS, 0, stream>>>(a);
+        auto kernel = format == B200_SGEMM_NVFP4
+                          ? (vector ? dequantize_kernel<B200_SGEMM_NVFP4, T> : dequantize_unaligned_kernel<B200_SGEMM_NVFP4, T>)
+                          : (vector ? dequantize_kernel<B200_SGEMM_MXFP4, T> : dequantize_unaligned_kernel<B200_SGEMM_MXFP4, T>);
+        kernel<<<grid, Q_THREADS, 0, stream>>>(a);
         return (int)cudaPeekAtLastError();
     });
 }
