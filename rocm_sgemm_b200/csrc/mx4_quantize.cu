@@ -113,25 +113,56 @@ __device__ __forceinline__ void scaled16(float2 (&y)[Q_LANE_K / 2], const float 
         y[i] = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(f, f));
 }
 
-// the values behind the nibbles in which `low` and `high` differ, by exact comparison; again(i) is x[i]
-template<class Again>
-__device__ __forceinline__ unsigned settle(unsigned low, unsigned high, int first, const Scale& sc, const Global& G, Again again)
+// Sign of |x| minus the midpoint above code `code`: exact.
+__device__ __forceinline__ float beyond_midpoint(float x, unsigned code, const Scale& sc, const Global& G)
 {
-    for(unsigned left = low ^ high; left;)
+    const float mid = 0.5f * (e2m1_value(code) + e2m1_value(code + 1));
+    return fmaf(-(mid * sc.s), G.g, fabsf(x));
+}
+
+// Settles the nibbles in which `low` and `high` (one more) differ.  again(i) is x[i].
+//   FP32    one by one.
+//   FP16 and BF16, all at once: such an x lies within 2^-20 of t s g, so the quotient x / (t s), eleven bits over seven, is
+//           that close to g.  Two such quotients of one binade are at least 2^-18 apart, so all values of the matrix that need
+//           settling have the same quotient and lie on the same side, or all on their midpoints.
+template<class T, class Again>
+__device__ __forceinline__ uint2 settle(uint2 low, uint2 high, const Scale& sc, const Global& G, Again again)
+{
+    if(sizeof(T) == 2)
     {
-        const int      i    = (__ffs(left) - 1) >> 2;
-        const unsigned code = low >> (4 * i) & 7u; // and code + 1 is the other one
-        const float    mid  = 0.5f * (e2m1_value(code) + e2m1_value(code + 1));
-        const float    d    = fmaf(-(mid * sc.s), G.g, fabsf(again(first + i)));
-        if(d > 0.f || (d == 0.f && (code & 1u)))
-            low += 1u << (4 * i);
-        left &= ~(0xFu << (4 * i));
+        const bool     second = low.x == high.x;
+        const unsigned word = second ? low.y : low.x, left = second ? low.y ^ high.y : low.x ^ high.x;
+        const int      i = (__ffs(left) - 1) >> 2;
+        const float    d = beyond_midpoint(again(second ? 8 + i : i), word >> (4 * i) & 7u, sc, G);
+        if(d > 0.f)
+            return high;
+        if(d == 0.f) // each to the even one: up by one where the nibbles differ and the lower is odd
+        {
+            const unsigned x = low.x ^ high.x, y = low.y ^ high.y;
+            low.x += (x | x >> 1 | x >> 2) & low.x & 0x11111111u;
+            low.y += (y | y >> 1 | y >> 2) & low.y & 0x11111111u;
+        }
+        return low;
+    }
+#pragma unroll
+    for(int half = 0; half < 2; ++half)
+    {
+        unsigned& word = half ? low.y : low.x;
+        for(unsigned left = word ^ (half ? high.y : high.x); left;)
+        {
+            const int      i    = (__ffs(left) - 1) >> 2;
+            const unsigned code = word >> (4 * i) & 7u;
+            const float    d    = beyond_midpoint(again(8 * half + i), code, sc, G);
+            if(d > 0.f || (d == 0.f && (code & 1u)))
+                word += 1u << (4 * i);
+            left &= ~(0xFu << (4 * i));
+        }
     }
     return low;
 }
 
 // sixteen codes, eight bytes
-template<int FMT, class Again>
+template<int FMT, class T, class Again>
 __device__ __forceinline__ uint2 encode(const float (&x)[Q_LANE_K], const Scale& sc, const Global& G, Again again)
 {
     if(sc.inv == 0.f)
@@ -161,10 +192,7 @@ __device__ __forceinline__ uint2 encode(const float (&x)[Q_LANE_K], const Scale&
     scaled16(y, x, sc.inv * (1.f + 0x1p-21f));
     const uint2 high = codes16(y);
     if(low.x != high.x || low.y != high.y)
-    {
-        low.x = settle(low.x, high.x, 0, sc, G, again);
-        low.y = settle(low.y, high.y, 8, sc, G, again);
-    }
+        low = settle<T>(low, high, sc, G, again);
     return low;
 }
 
@@ -187,7 +215,7 @@ struct QArgs
     uint8_t*     scales;
     long long    ld, pitch;
     int          rows, source_rows, K, tiles, index_div;
-    int          vector; // base and pitch of X allow 32-byte loads
+    int          vector; // base and pitch of X allow loads of 32 (rows) or 4 bytes (columns)
 };
 
 // address of (row, block) in the scales
@@ -248,12 +276,16 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_c
     {
         const long long src = next;
         float           x[Q_LANE_K];
-#pragma unroll
-        for(int j = 0; j < Q_LANE_K; ++j)
+        if(vector)
         {
-            if(vector)
+#pragma unroll
+            for(int j = 0; j < Q_LANE_K; ++j)
                 x[j] = to_float(ahead[j / Vec32<T>::N].v[j % Vec32<T>::N]);
-            else
+        }
+        else
+        {
+#pragma unroll
+            for(int j = 0; j < Q_LANE_K; ++j)
                 x[j] = src >= 0 && k0 + j < a.K ? to_float(X[src * a.ld + k0 + j]) : 0.f;
         }
         next = r + Q_THREADS / 32 < Q_ROWS ? source(r + Q_THREADS / 32) : -1;
@@ -266,7 +298,7 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_c
             if(FMT == B200_SGEMM_MXFP4)
                 amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1)); // NaN orders above infinity
             sc            = FMT == B200_SGEMM_NVFP4 ? scale_nvfp4(amax, G) : scale_mxfp4(amax);
-            const uint2 c = encode<FMT>(x, sc, G, [&](int i) { return to_float(X[src * a.ld + k0 + i]); });
+            const uint2 c = encode<FMT, T>(x, sc, G, [&](int i) { return to_float(X[src * a.ld + k0 + i]); });
             if(k0 < 2 * a.pitch)
                 *reinterpret_cast<uint2*>(a.codes + (row0 + r) * a.pitch + k0 / 2) = c;
         }
@@ -285,56 +317,86 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_c
     }
 }
 
-// Row-contiguous source (a col-major A, a row-major B).  One CTA: a band of 128 rows x 128 k; a thread takes one row and
-// 64 k, lanes take neighbouring rows, so every load is contiguous over the warp and a thread has whole blocks in
-// registers; its 32 code bytes are one sector.
+// Row-contiguous source (a col-major A, a row-major B).  One CTA: a band of 128 rows x 128 k.  A thread takes one row (FP32) or
+// two neighbours (16 bits, one load of both), 32 k at a time; lanes take neighbouring rows, so a warp loads 128 contiguous
+// bytes of a k, and a thread has whole blocks in registers.  (One row per thread of 16-bit types: 64 bytes a load, 270 us for
+// 16384 x 8192 BF16.)
 template<int FMT, class T>
 __global__ void __launch_bounds__(Q_THREADS) quantize_cols_kernel(const __grid_constant__ QArgs a)
 {
     constexpr int   BLOCK = FMT == B200_SGEMM_NVFP4 ? 16 : 32;
+    constexpr int   R = 4 / sizeof(T), SPAN = 64 / R; // rows and k of a thread
     const int       k_ctas = (a.K + Q_COL_K - 1) / Q_COL_K;
     const int       band = blockIdx.x / k_ctas, kc = blockIdx.x - band * k_ctas;
-    const int       r = threadIdx.x & (MX4_BAND - 1), half = threadIdx.x / MX4_BAND;
-    const long long row = (long long)band * MX4_BAND + r;
-    const T*        X   = static_cast<const T*>(a.x);
-    const Global    G   = load_global(a.global);
-    const bool      in  = row < a.rows;
-    unsigned        word = 0; // the scales of the thread's 64 k
+    const int       pair = threadIdx.x % (MX4_BAND / R), part = threadIdx.x / (MX4_BAND / R);
+    const long long row0 = (long long)band * MX4_BAND + pair * R;
+    const T*        X    = static_cast<const T*>(a.x);
+    const Global    G    = load_global(a.global);
 #pragma unroll
-    for(int j = 0; j < 2; ++j) // 32 k at a time
+    for(int j = 0; j < SPAN / 32; ++j)
     {
-        const int k0 = kc * Q_COL_K + half * 64 + j * 32;
-        float     x[2][Q_LANE_K];
+        const int k0 = kc * Q_COL_K + part * SPAN + j * 32;
+        if(k0 >= a.tiles * 4 * BLOCK)
+            break;
+        uint32_t raw[32];
+        if(a.vector && row0 + R <= a.rows) // both rows (the only one) and aligned
+        {
 #pragma unroll
-        for(int i = 0; i < 32; ++i)
-            x[i / 16][i % 16] = in && k0 + i < a.K ? to_float(X[(long long)(k0 + i) * a.ld + row]) : 0.f;
-        unsigned amax[2] = {amax16(x[0]), amax16(x[1])};
-        Scale    sc[2];
-        if(FMT == B200_SGEMM_MXFP4)
-            sc[0] = sc[1] = scale_mxfp4(max(amax[0], amax[1]));
+            for(int i = 0; i < 32; ++i)
+                raw[i] = k0 + i < a.K ? __ldg(reinterpret_cast<const uint32_t*>(X + (long long)(k0 + i) * a.ld + row0)) : 0u;
+        }
         else
         {
-            sc[0] = scale_nvfp4(amax[0], G);
-            sc[1] = scale_nvfp4(amax[1], G);
+#pragma unroll
+            for(int i = 0; i < 32; ++i)
+            {
+                T v[R];
+#pragma unroll
+                for(int m = 0; m < R; ++m)
+                    v[m] = row0 + m < a.rows && k0 + i < a.K ? X[(long long)(k0 + i) * a.ld + row0 + m] : from_float<T>(0.f);
+                if constexpr(R == 1)
+                    raw[i] = __float_as_uint(to_float(v[0]));
+                else
+                    raw[i] = *reinterpret_cast<const uint16_t*>(&v[0]) | (uint32_t)*reinterpret_cast<const uint16_t*>(&v[R - 1]) << 16;
+            }
         }
-        auto        again = [&](int i) { return to_float(X[(long long)(k0 + i) * a.ld + row]); };
-        const uint2 lo = encode<FMT>(x[0], sc[0], G, again);
-        const uint2 hi = encode<FMT>(x[1], sc[1], G, [&](int i) { return again(16 + i); });
-        if(in && k0 < 2 * a.pitch)
-            *reinterpret_cast<uint4*>(a.codes + row * a.pitch + k0 / 2) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        if(FMT == B200_SGEMM_NVFP4)
-            word |= (sc[0].byte | sc[1].byte << 8) << (16 * j);
-        else
-            word |= sc[0].byte << (8 * j);
-    }
-    const int block = (kc * Q_COL_K + half * 64) / BLOCK;
-    if(block >> 2 < a.tiles)
-    {
-        uint8_t* to = a.scales + scale_at(row, block, a.tiles);
-        if(FMT == B200_SGEMM_NVFP4)
-            *reinterpret_cast<uint32_t*>(to) = in ? word : 0u;
-        else
-            *reinterpret_cast<uint16_t*>(to) = in ? (uint16_t)word : (uint16_t)0;
+#pragma unroll
+        for(int m = 0; m < R; ++m)
+        {
+            const long long row = row0 + m;
+            float           x[2][Q_LANE_K];
+#pragma unroll
+            for(int i = 0; i < 32; ++i)
+            {
+                if constexpr(R == 1)
+                    x[i / 16][i % 16] = __uint_as_float(raw[i]);
+                else
+                {
+                    const uint16_t bits = (uint16_t)(raw[i] >> (16 * m));
+                    x[i / 16][i % 16]   = to_float(*reinterpret_cast<const T*>(&bits));
+                }
+            }
+            const unsigned amax[2] = {amax16(x[0]), amax16(x[1])};
+            Scale          sc[2];
+            if(FMT == B200_SGEMM_MXFP4)
+                sc[0] = sc[1] = scale_mxfp4(max(amax[0], amax[1]));
+            else
+            {
+                sc[0] = scale_nvfp4(amax[0], G);
+                sc[1] = scale_nvfp4(amax[1], G);
+            }
+            auto        again = [&](int i) { return to_float(X[(long long)(k0 + i) * a.ld + row]); };
+            const uint2 lo = encode<FMT, T>(x[0], sc[0], G, again);
+            const uint2 hi = encode<FMT, T>(x[1], sc[1], G, [&](int i) { return again(16 + i); });
+            const bool  in = row < a.rows;
+            if(in && k0 < 2 * a.pitch)
+                *reinterpret_cast<uint4*>(a.codes + row * a.pitch + k0 / 2) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            uint8_t* to = a.scales + scale_at(row, k0 / BLOCK, a.tiles);
+            if(FMT == B200_SGEMM_NVFP4)
+                *reinterpret_cast<uint16_t*>(to) = in ? (uint16_t)(sc[0].byte | sc[1].byte << 8) : (uint16_t)0;
+            else
+                *to = in ? (uint8_t)sc[0].byte : (uint8_t)0;
+        }
     }
 }
 
@@ -521,7 +583,8 @@ extern "C" int b200_sgemm_mx4_quantize(int format, int layout, int type, const v
     a.K           = (int)K;
     a.tiles       = (int)mx4_tiles(format, K);
     a.index_div   = index_div;
-    a.vector      = !misaligned(X, 32) && ldx * type_bytes(type) % 32 == 0;
+    const size_t access = row_major ? 32 : 4; // bytes of a load
+    a.vector            = !misaligned(X, access) && ldx * type_bytes(type) % access == 0;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
