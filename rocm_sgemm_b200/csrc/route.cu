@@ -18,6 +18,7 @@ using namespace sgemm_b200;
 
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS   = SORT_THREADS / 32;
+constexpr int SORT_CTAS    = 8; // of a cluster, at most
 constexpr int MAX_EXPERTS  = 1024; // one thread each in the scan
 
 struct SortArgs
@@ -27,7 +28,8 @@ struct SortArgs
     int*       counts;
     int*       slot_row;
     int*       row_slot;
-    int        slots, experts, align, rows, ctas, per_warp;
+    int        slots, experts, align, rows, ctas, bits; // bits that tell experts and -1 apart
+    int        warps, per_warp;                         // warps of a CTA that hold slots, and how many each
 };
 
 __device__ __forceinline__ int expert_of(const SortArgs& a, int slot)
@@ -51,34 +53,62 @@ __device__ __forceinline__ int ld_cluster_int(const int* p, int rank)
 
 __global__ void __launch_bounds__(SORT_THREADS, 1) route_sort_kernel(const __grid_constant__ SortArgs a)
 {
-    extern __shared__ int before[]; // [SORT_WARPS][experts]: slots of an expert in this CTA's earlier warps
-    __shared__ int total[MAX_EXPERTS], start[MAX_EXPERTS], warp_sum[SORT_WARPS], end_row;
+    extern __shared__ int before[]; // [warps][experts]: slots of an expert in this CTA's earlier warps
+    __shared__ int total[MAX_EXPERTS], start[MAX_EXPERTS], warp_sum[SORT_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = threadIdx.x;
     const int rank = a.ctas > 1 ? (int)(blockIdx.x % a.ctas) : 0;
     int*      mine = before + warp * a.experts;
-    const long long begin = (long long)(rank * SORT_WARPS + warp) * a.per_warp; // the last warps' range may lie behind the slots
-    const int       count = (int)max(0ll, min((long long)a.per_warp, a.slots - begin));
+    // the range of the last warps may lie behind the slots
+    const long long begin = (long long)(rank * a.warps + warp) * a.per_warp;
+    const int       count = warp < a.warps ? (int)max(0ll, min((long long)a.per_warp, a.slots - begin)) : 0;
 
-    for(int i = lane; i < a.experts; i += 32)
-        mine[i] = 0;
-    __syncwarp();
-    for(int i = 0; i < count; i += 32)
+    // f(expert, position in the range) for 32 slots at a time; the experts of four such batches are fetched together (one by one,
+    // 32768 slots took 10.9 us)
+    auto each_batch = [&](auto f) {
+        for(int i0 = 0; i0 < count; i0 += 128)
+        {
+            int x[4];
+#pragma unroll
+            for(int b = 0; b < 4; ++b)
+                x[b] = i0 + b * 32 + lane < count ? expert_of(a, (int)begin + i0 + b * 32 + lane) : -1;
+#pragma unroll
+            for(int b = 0; b < 4; ++b)
+                if(i0 + b * 32 < count)
+                    f(x[b], i0 + b * 32 + lane);
+        }
+    };
+
+    if(warp < a.warps)
     {
-        const int      x    = i + lane < count ? expert_of(a, (int)begin + i + lane) : -1;
-        const unsigned same = __match_any_sync(0xFFFFFFFFu, x);
-        if(x >= 0 && (same & ((1u << lane) - 1u)) == 0)
-            mine[x] += __popc(same);
+        for(int i = lane; i < a.experts; i += 32)
+            mine[i] = 0;
+        __syncwarp();
+        each_batch([&](int x, int) {
+            if(x >= 0)
+                atomicAdd(mine + x, 1); // of this warp alone, and a sum of ones: the order does not matter
+        });
         __syncwarp();
     }
+    // every row without a slot until one is placed there, which is behind the barriers below
+    for(long long row = rank * SORT_THREADS + threadIdx.x; row < a.rows; row += a.ctas * SORT_THREADS)
+        a.row_slot[row] = -1;
     __syncthreads();
     if(e < a.experts)
     {
         int sum = 0;
-        for(int w = 0; w < SORT_WARPS; ++w)
+        for(int w0 = 0; w0 < a.warps; w0 += 8)
         {
-            const int n = before[w * a.experts + e];
-            before[w * a.experts + e] = sum;
-            sum += n;
+            int n[8];
+#pragma unroll
+            for(int w = 0; w < 8; ++w)
+                n[w] = w0 + w < a.warps ? before[(w0 + w) * a.experts + e] : 0;
+#pragma unroll
+            for(int w = 0; w < 8; ++w)
+            {
+                if(w0 + w < a.warps)
+                    before[(w0 + w) * a.experts + e] = sum;
+                sum += n[w];
+            }
         }
         total[e] = sum;
     }
@@ -86,12 +116,18 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) route_sort_kernel(const __gri
         cluster_sync();
     int all = 0, earlier = 0;
     if(e < a.experts)
-        for(int r = 0; r < a.ctas; ++r)
+    {
+        int n[SORT_CTAS]; // all in flight at once
+#pragma unroll
+        for(int r = 0; r < SORT_CTAS; ++r)
+            n[r] = a.ctas == 1 ? (r == 0 ? total[e] : 0) : (r < a.ctas ? ld_cluster_int(total + e, r) : 0);
+#pragma unroll
+        for(int r = 0; r < SORT_CTAS; ++r)
         {
-            const int n = a.ctas > 1 ? ld_cluster_int(total + e, r) : total[e];
-            earlier += r < rank ? n : 0;
-            all += n;
+            earlier += r < rank ? n[r] : 0;
+            all += n[r];
         }
+    }
     // exclusive sum of the experts' rounded-up rows
     const int padded = (all + a.align - 1) / a.align * a.align;
     int       upto   = padded;
@@ -128,35 +164,26 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) route_sort_kernel(const __gri
                 a.offsets[a.experts] = first + padded;
         }
     }
-    if(e == a.experts - 1)
-        end_row = first + padded;
     __syncthreads();
-    for(int i = 0; i < count; i += 32)
-    {
-        const int      slot = (int)begin + i + lane;
-        const bool     in   = i + lane < count;
-        const int      x    = in ? expert_of(a, slot) : -1;
-        const unsigned same = __match_any_sync(0xFFFFFFFFu, x);
+    each_batch([&](int x, int i) {
+        unsigned same = 0xFFFFFFFFu; // lanes with the same expert: those that agree in every bit (the match instruction is slower)
+        for(int bit = 0; bit < a.bits; ++bit)
+        {
+            const bool     one = x >> bit & 1;
+            const unsigned set = __ballot_sync(0xFFFFFFFFu, one);
+            same &= one ? set : ~set;
+        }
         const unsigned low  = same & ((1u << lane) - 1u);
-        int            row  = -1;
-        if(x >= 0)
-            row = start[x] + mine[x] + __popc(low);
+        const int      slot = (int)begin + i, row = x >= 0 ? start[x] + mine[x] + __popc(low) : -1;
         __syncwarp();
         if(x >= 0 && low == 0)
             mine[x] += __popc(same);
         __syncwarp();
-        if(in)
+        if(i < count)
             a.slot_row[slot] = row;
         if(row >= 0)
             a.row_slot[row] = slot;
-    }
-    // rows without a slot: behind each expert's, and behind the last expert
-    const int stride = a.ctas * SORT_THREADS, at = rank * SORT_THREADS + threadIdx.x;
-    if(a.align > 1 && e < a.experts && e % a.ctas == rank)
-        for(int row = first + all; row < first + padded; ++row)
-            a.row_slot[row] = -1;
-    for(long long row = (long long)end_row + at; row < a.rows; row += stride)
-        a.row_slot[row] = -1;
+    });
     if(a.ctas > 1)
         cluster_sync(); // nobody leaves while its totals are being read
 }
@@ -198,75 +225,121 @@ struct RowArgs
     int          pieces; // pieces of a row, in units of a warp's step
 };
 
-constexpr int R_UNROLL = 4; // pieces of one lane in flight
+// How a warp takes a token's row: UNROLL x 32 pieces of it, and (combine) ROWS of the slots' rows fetched at once.  Many tokens: 4
+// pieces and one row, which leaves registers for many warps; few, where one warp's latency is all there is: 1 piece and 8 rows.
+// Combine of 8192 tokens x 4 x 4096 BF16 took 51 us with (4, 1), 55 us with (2, 4), 72 us with (1, 8); of 64 tokens x 8
+// 4.9 us with (4, 1), 3.1 us with (2, 4), 2.6 us with (1, 8).
 
-__device__ __forceinline__ long long row_of(const RowArgs& a, long long slot)
+__device__ __forceinline__ int row_of(const RowArgs& a, long long slot)
 {
     const int r = __ldg(a.slot_row + slot);
     return (unsigned)r < (unsigned)a.rows ? r : -1;
 }
 
-// one warp: R_UNROLL x 32 pieces of one token's row
-template<class T, int N>
+template<class T, int N, int UNROLL>
 __global__ void __launch_bounds__(R_THREADS) route_dispatch_kernel(const __grid_constant__ RowArgs a)
 {
+    const int       lane = threadIdx.x & 31;
     const long long unit = (long long)blockIdx.x * (R_THREADS / 32) + (threadIdx.x >> 5);
     const long long t    = unit / a.pieces;
     if(t >= a.tokens)
         return;
-    const int c0 = ((int)(unit - t * a.pieces) * R_UNROLL * 32 + (threadIdx.x & 31)) * N;
+    const int c0 = ((int)(unit - t * a.pieces) * UNROLL * 32 + lane) * N;
     const T*  x  = static_cast<const T*>(a.x) + t * a.ldx;
-    Piece<T, N> p[R_UNROLL];
+    Piece<T, N> p[UNROLL];
 #pragma unroll
-    for(int u = 0; u < R_UNROLL; ++u)
+    for(int u = 0; u < UNROLL; ++u)
         if(c0 + u * 32 * N < a.width)
             p[u].load(x + c0 + u * 32 * N);
-    for(int j = 0; j < a.top_k; ++j)
+    for(int j0 = 0; j0 < a.top_k; j0 += 32)
     {
-        const long long r = row_of(a, t * a.top_k + j);
-        if(r < 0)
-            continue;
-        T* to = static_cast<T*>(a.out) + r * a.ldo;
+        const int mine = j0 + lane < a.top_k ? row_of(a, t * a.top_k + j0 + lane) : -1;
+        for(int j = 0; j < min(32, a.top_k - j0); ++j)
+        {
+            const int r = __shfl_sync(0xFFFFFFFFu, mine, j);
+            if(r < 0)
+                continue;
+            T* to = static_cast<T*>(a.out) + r * a.ldo;
 #pragma unroll
-        for(int u = 0; u < R_UNROLL; ++u)
-            if(c0 + u * 32 * N < a.width)
-                p[u].store(to + c0 + u * 32 * N);
+            for(int u = 0; u < UNROLL; ++u)
+                if(c0 + u * 32 * N < a.width)
+                    p[u].store(to + c0 + u * 32 * N);
+        }
     }
 }
 
-template<class T, int N>
+template<class T, int N, int UNROLL, int ROWS>
 __global__ void __launch_bounds__(R_THREADS) route_combine_kernel(const __grid_constant__ RowArgs a)
 {
+    const int       lane = threadIdx.x & 31;
     const long long unit = (long long)blockIdx.x * (R_THREADS / 32) + (threadIdx.x >> 5);
     const long long t    = unit / a.pieces;
     if(t >= a.tokens)
         return;
-    const int c0 = ((int)(unit - t * a.pieces) * R_UNROLL * 32 + (threadIdx.x & 31)) * N;
-    float     sum[R_UNROLL][N] = {};
-    for(int j = 0; j < a.top_k; ++j)
-    {
-        const long long r = row_of(a, t * a.top_k + j);
-        if(r < 0)
-            continue;
-        const float w = a.weights ? __ldg(a.weights + t * a.top_k + j) : 1.f;
-        const T*    y = static_cast<const T*>(a.x) + r * a.ldx;
-        Piece<T, N> p[R_UNROLL];
+    const int c0 = ((int)(unit - t * a.pieces) * UNROLL * 32 + lane) * N;
+    float     sum[UNROLL][N] = {};
+    auto add = [&](const Piece<T, N>(&p)[UNROLL], float w) {
 #pragma unroll
-        for(int u = 0; u < R_UNROLL; ++u)
-            if(c0 + u * 32 * N < a.width)
-                p[u].load(y + c0 + u * 32 * N);
-#pragma unroll
-        for(int u = 0; u < R_UNROLL; ++u)
+        for(int u = 0; u < UNROLL; ++u)
             if(c0 + u * 32 * N < a.width)
             {
 #pragma unroll
                 for(int i = 0; i < N; ++i)
                     sum[u][i] = fmaf(w, to_float(p[u].v[i]), sum[u][i]);
             }
+    };
+    auto fetch = [&](Piece<T, N>(&p)[UNROLL], int r) {
+        const T* y = static_cast<const T*>(a.x) + r * a.ldx;
+#pragma unroll
+        for(int u = 0; u < UNROLL; ++u)
+            if(c0 + u * 32 * N < a.width)
+                p[u].load(y + c0 + u * 32 * N);
+    };
+    if constexpr(ROWS == 1)
+    {
+        for(int j = 0; j < a.top_k; ++j)
+        {
+            const int r = row_of(a, t * a.top_k + j);
+            if(r < 0)
+                continue;
+            const float w = a.weights ? __ldg(a.weights + t * a.top_k + j) : 1.f;
+            Piece<T, N> p[UNROLL];
+            fetch(p, r);
+            add(p, w);
+        }
+    }
+    else
+    {
+        for(int j0 = 0; j0 < a.top_k; j0 += 32) // the rows and weights of 32 slots at once
+        {
+            const bool  slot   = j0 + lane < a.top_k;
+            const int   mine   = slot ? row_of(a, t * a.top_k + j0 + lane) : -1;
+            const float weight = slot && a.weights ? __ldg(a.weights + t * a.top_k + j0 + lane) : 1.f;
+            const int   n      = min(32, a.top_k - j0);
+            for(int j1 = 0; j1 < n; j1 += ROWS) // fetched together, added in order
+            {
+                int         r[ROWS];
+                Piece<T, N> p[ROWS][UNROLL];
+#pragma unroll
+                for(int j = 0; j < ROWS; ++j)
+                {
+                    r[j] = j1 + j < n ? __shfl_sync(0xFFFFFFFFu, mine, j1 + j) : -1;
+                    if(r[j] >= 0)
+                        fetch(p[j], r[j]);
+                }
+#pragma unroll
+                for(int j = 0; j < ROWS; ++j)
+                {
+                    const float w = __shfl_sync(0xFFFFFFFFu, weight, (j1 + j) & 31);
+                    if(r[j] >= 0)
+                        add(p[j], w);
+                }
+            }
+        }
     }
     T* to = static_cast<T*>(a.out) + t * a.ldo;
 #pragma unroll
-    for(int u = 0; u < R_UNROLL; ++u)
+    for(int u = 0; u < UNROLL; ++u)
         if(c0 + u * 32 * N < a.width)
         {
             Piece<T, N> p;
@@ -289,8 +362,8 @@ __global__ void __launch_bounds__(R_THREADS) route_backward_kernel(const __grid_
     for(int j0 = 0; j0 < a.top_k; j0 += B_SLOTS)
     {
         const int n = min(B_SLOTS, a.top_k - j0);
-        long long row[B_SLOTS];
-        float     w[B_SLOTS], dot[B_SLOTS];
+        int   row[B_SLOTS];
+        float w[B_SLOTS], dot[B_SLOTS];
 #pragma unroll
         for(int j = 0; j < B_SLOTS; ++j)
         {
@@ -368,13 +441,26 @@ bool sizes_ok(size_t tokens, size_t top_k, size_t width, size_t rows)
 {
     return tokens <= MAX_EXTENT && top_k <= MAX_EXTENT && tokens * top_k <= MAX_EXTENT && width <= MAX_EXTENT && rows <= MAX_EXTENT;
 }
-// CTAs for one warp per R_UNROLL x 32 pieces of N elements; 0: more than a grid holds
-unsigned warp_grid(size_t tokens, int* pieces, size_t width, int n)
+// CTAs for one warp per `unroll` x 32 pieces of n elements; 0: more than a grid holds
+unsigned warp_grid(const RowArgs& a, int* pieces, int n, int unroll)
 {
-    const size_t per  = (size_t)R_UNROLL * 32 * n;
-    *pieces           = (int)((width + per - 1) / per);
-    const size_t ctas = (tokens * (size_t)*pieces + R_THREADS / 32 - 1) / (R_THREADS / 32);
+    const size_t per  = (size_t)unroll * 32 * n;
+    *pieces           = (int)(((size_t)a.width + per - 1) / per);
+    const size_t ctas = ((size_t)a.tokens * *pieces + R_THREADS / 32 - 1) / (R_THREADS / 32);
     return ctas > 0x7fffffffull ? 0u : (unsigned)ctas;
+}
+// launches f(grid, many) for the two ways of taking a row: `many` from one wave of 148 SMs x 8 CTAs on
+template<class F>
+int with_grid(RowArgs& a, int n, F f)
+{
+    unsigned   grid = warp_grid(a, &a.pieces, n, 4);
+    const bool many = grid >= 148u * 8u || grid == 0;
+    if(!many)
+        grid = warp_grid(a, &a.pieces, n, 1);
+    if(!grid)
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    f(grid, many);
+    return (int)cudaPeekAtLastError();
 }
 } // namespace
 
@@ -408,10 +494,14 @@ extern "C" int b200_sgemm_route_sort(const int* expert_ids, size_t tokens, size_
     a.experts  = (int)experts;
     a.align    = (int)align;
     a.rows     = (int)rows;
-    a.ctas     = a.slots <= 4096 ? 1 : (a.slots <= 16384 ? 4 : 8);
-    const int warps = a.ctas * SORT_WARPS;
-    a.per_warp      = ((a.slots + warps - 1) / warps + 31) / 32 * 32;
-    const size_t smem = (size_t)SORT_WARPS * experts * sizeof(int);
+    a.ctas     = a.slots <= 1024 ? 1 : (a.slots <= 4096 ? 4 : SORT_CTAS);
+    a.bits = 1;
+    while((1 << a.bits) <= a.experts)
+        ++a.bits;
+    const int per_cta = (a.slots + a.ctas - 1) / a.ctas;
+    a.warps           = per_cta >= SORT_THREADS ? SORT_WARPS : (per_cta + 31) / 32;
+    a.per_warp        = ((per_cta + a.warps - 1) / a.warps + 31) / 32 * 32;
+    const size_t smem = (size_t)a.warps * experts * sizeof(int);
     cudaError_t  e    = cudaFuncSetAttribute(route_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if(e != cudaSuccess)
         return (int)e;
@@ -454,11 +544,10 @@ extern "C" int b200_sgemm_route_dispatch(int type, const void* X, size_t tokens,
     a.width    = (int)width;
     a.rows     = (int)rows;
     return with_pieces(type, rows_vector(type, X, ldx) && rows_vector(type, Xs, lds), width, [&](auto t, auto n) {
-        const unsigned grid = warp_grid(tokens, &a.pieces, width, n());
-        if(!grid)
-            return B200_SGEMM_UNSUPPORTED_SIZE;
-        route_dispatch_kernel<decltype(t), n()><<<grid, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
-        return (int)cudaPeekAtLastError();
+        return with_grid(a, n(), [&](unsigned grid, bool many) {
+            auto kernel = many ? route_dispatch_kernel<decltype(t), n(), 4> : route_dispatch_kernel<decltype(t), n(), 1>;
+            kernel<<<grid, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
+        });
     });
 }
 
@@ -488,11 +577,10 @@ extern "C" int b200_sgemm_route_combine(int type, const void* Y, size_t rows, si
     a.width    = (int)width;
     a.rows     = (int)rows;
     return with_pieces(type, rows_vector(type, Y, ldy) && rows_vector(type, out, ldo), width, [&](auto t, auto n) {
-        const unsigned grid = warp_grid(tokens, &a.pieces, width, n());
-        if(!grid)
-            return B200_SGEMM_UNSUPPORTED_SIZE;
-        route_combine_kernel<decltype(t), n()><<<grid, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
-        return (int)cudaPeekAtLastError();
+        return with_grid(a, n(), [&](unsigned grid, bool many) {
+            auto kernel = many ? route_combine_kernel<decltype(t), n(), 4, 1> : route_combine_kernel<decltype(t), n(), 1, 8>;
+            kernel<<<grid, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
+        });
     });
 }
 
