@@ -6,10 +6,10 @@
 // Both operands are K-contiguous, so either can take either side of a tile.  The kernel knows a LANE operand P (128 rows
 // of it on the 128 lanes of tensor memory) and a COLUMN operand Q (BN rows of it as columns):
 //   lanes    the dimension along which C is contiguous, so that a warp stores 32 neighbours of C at once; for few tokens
-//            that is the weights, and the tokens cost BN = 32 columns instead of a tile of 128 rows
+//            that is the weights, and the tokens cost 32 or 64 columns instead of a tile of 128 rows
 //   columns  the other one; the rows of the groups in the grouped product
 //
-// Tiles.  128 lanes x 32, 64 or 128 columns by one CTA, or 256 lanes x 128 or 256 columns by a pair of CTAs on
+// Tiles.  128 lanes x 64 or 128 columns by one CTA, or 256 lanes x 128 or 256 columns by a pair of CTAs on
 // neighbouring SMs: each holds 128 of the lanes, half of Q's rows and all of Q's scales, and the first one issues for both.
 // A pair reads half of Q from the L2 and from shared memory and issues half the scale copies per product.
 //
@@ -63,14 +63,15 @@ struct GLayout
 {
     static constexpr int    TILE_P      = PAIR * G_LANES;
     static constexpr int    Q_ROWS      = BN / PAIR;                     // of this CTA
+    static constexpr int    Q_BOX       = BN == 64 ? 32 : Q_ROWS;        // rows of one copy; a tile of up to 32 rows takes one of two
     static constexpr int    Q_BANDS     = (BN + MX4_BAND - 1) / MX4_BAND; // bands of scales that a column tile touches
     static constexpr int    TILES       = G_KBLOCK / (4 * mx4_block(FMT)); // scale tiles of a band in a stage
     static constexpr int    P_BYTES     = G_LANES * G_ROW_BYTES;
     static constexpr int    Q_BYTES     = Q_ROWS * G_ROW_BYTES;
     static constexpr int    P_SCALES    = TILES * MX4_TILE_BYTES;
     static constexpr int    Q_SCALES    = Q_BANDS * P_SCALES;
-    static constexpr int    FILL_BYTES  = P_BYTES + Q_BYTES + P_SCALES + Q_SCALES;
-    static constexpr int    STAGE_BYTES = (FILL_BYTES + 1023) / 1024 * 1024;
+    static constexpr int    BOX_BYTES   = Q_BOX * G_ROW_BYTES;
+    static constexpr int    STAGE_BYTES = (P_BYTES + Q_BYTES + P_SCALES + Q_SCALES + 1023) / 1024 * 1024;
     static constexpr int    SLOT_COLS   = 4 * TILES * (1 + Q_BANDS); // tensor-memory columns of a stage's scales
     static constexpr int    BY_SMEM     = (216 * 1024) / STAGE_BYTES;
     static constexpr int    BY_TMEM     = (G_TMEM_COLS - G_SCALE_COL) / SLOT_COLS;
@@ -80,6 +81,7 @@ struct GLayout
     static constexpr size_t SMEM_BYTES  = size_t(STAGES) * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers, misc*/;
     static_assert(8 * BARRIERS + 16 <= 256, "barrier area");
     static_assert(ACCS * BN <= G_SCALE_COL, "tensor memory");
+    static_assert(BN % 64 == 0 && SLOT_COLS % 4 == 0 && TILES % 2 == 0, "scales start on an even column");
     static_assert(SMEM_BYTES + (G_MAX_GROUPS + 1) * 4 <= 227 * 1024, "shared memory");
     static_assert(PAIR > 1 || BN * G_LANES * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile lie in the ring");
 };
@@ -165,10 +167,10 @@ __device__ __forceinline__ uint64_t scales_desc(uint32_t addr)
 }
 // block-scaled product: e2m1 operands (1), both K-major, N >> 3, scale type (0 e4m3, 1 e8m0), M >> 4; which bytes of the
 // 32-bit scale words an instruction takes is added by the issuer (bits 4-5 for Q, 29-30 for P)
-template<int FMT, int BN, int PAIR>
-__device__ __forceinline__ constexpr uint32_t mx4_idesc()
+template<int FMT, int PAIR>
+__device__ __forceinline__ constexpr uint32_t mx4_idesc(uint32_t n)
 {
-    return (1u << 7) | (1u << 10) | (uint32_t(BN >> 3) << 17) | (FMT == B200_SGEMM_MXFP4 ? 1u << 23 : 0u)
+    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (FMT == B200_SGEMM_MXFP4 ? 1u << 23 : 0u)
            | (uint32_t(PAIR * G_LANES >> 4) << 24);
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -372,56 +374,95 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
     const int split = a.split, shared_by = PAIR * split; // CTAs of the cluster
     const int rank  = shared_by > 1 ? (int)(blockIdx.x % shared_by) : 0;
     const int lane0 = PAIR > 1 ? rank * G_LANES : 0; // this CTA's first lane in the tile
-    if(threadIdx.x == 0)
+    const int first = blockIdx.x / shared_by, stride = gridDim.x / shared_by;
+    const int part  = PAIR > 1 ? 0 : rank; // this CTA's range of K
+    const int kb0 = (int)((long long)a.kblocks * part / split), kb1 = (int)((long long)a.kblocks * (part + 1) / split);
+    // one stage of a tile: codes and scales of K block kb
+    auto fill = [&](const Tile& t, int kb, int s) {
+        const uint32_t st  = base + s * L::STAGE_BYTES;
+        const uint32_t bar = PAIR > 1 ? cluster_addr(full(s), 0) : full(s);
+        const bool     whole = L::Q_BOX == L::Q_ROWS || t.q0 + L::Q_BOX < t.q_end; // or the first box alone
+        if(rank == 0 || PAIR == 1)
+            mbar_arrive_expect_tx(full(s), PAIR * (L::P_BYTES + (whole ? L::Q_BYTES : L::BOX_BYTES) + L::P_SCALES + L::Q_SCALES));
+        load_codes<PAIR>(st, &maps.p, kb * G_ROW_BYTES, t.group * a.np + t.p0 + lane0, bar);
+        load_codes<PAIR>(st + L::P_BYTES, &maps.q, kb * G_ROW_BYTES, t.q0 + (PAIR > 1 ? rank * L::Q_ROWS : 0), bar);
+        if(L::Q_BOX < L::Q_ROWS && whole)
+            load_codes<PAIR>(st + L::P_BYTES + L::BOX_BYTES, &maps.q, kb * G_ROW_BYTES, t.q0 + L::Q_BOX, bar);
+        load_scales<PAIR>(st + L::P_BYTES + L::Q_BYTES, &maps.scales_p, kb * L::TILES, t.group * a.bands_p + (t.p0 + lane0) / MX4_BAND, bar);
+        load_scales<PAIR>(st + L::P_BYTES + L::Q_BYTES + L::P_SCALES, &maps.scales_q, kb * L::TILES, t.q0 / MX4_BAND, bar);
+    };
+    int filled = 0; // stages that are on their way before the rest of the CTA is ready
+    if(warp == G_TMA_WARP)
     {
-        for(int s = 0; s < STAGES; ++s)
+        if(lane < 4) // the four descriptors at once: each costs a trip to memory
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.p + lane)) : "memory");
+        if(lane == 0)
         {
-            mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
+            for(int s = 0; s < STAGES; ++s)
+            {
+                mbar_init(full(s), 1);
+                mbar_init(empty(s), 1);
+            }
+            for(int b = 0; b < 2; ++b)
+            {
+                mbar_init(acc_full(b), 1);
+                mbar_init(acc_empty(b), PAIR * G_EPILOGUE / 32);
+            }
+            mbar_init(drained, 1);
+            *abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        for(int b = 0; b < 2; ++b)
+        __syncwarp();
+        if(PAIR == 1 && a.groups == 0) // nothing to wait for: this CTA's first tile and its barriers are known
         {
-            mbar_init(acc_full(b), 1);
-            mbar_init(acc_empty(b), PAIR * G_EPILOGUE / 32);
+            const Tile t      = tile_at<BN, L::TILE_P>(a, nullptr, first);
+            const bool issuer = elect_one();
+            filled            = min(STAGES, kb1 - kb0);
+            for(int i = 0; i < filled; ++i)
+                if(issuer)
+                    fill(t, kb0 + i, i);
+            __syncwarp();
         }
-        mbar_init(drained, 1);
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if(warp == G_MMA_WARP)
     {
         tmem_alloc<PAIR>((uint32_t)__cvta_generic_to_shared(tmem_slot), G_TMEM_COLS);
         tmem_relinquish<PAIR>();
     }
-    if(warp == G_TMA_WARP && a.groups) // column tiles before each group
+    if(a.groups) // column tiles before each group
     {
-        int sum = 0;
-        for(int e0 = 0; e0 < a.groups; e0 += 32)
+        for(int e = threadIdx.x; e < a.groups; e += G_THREADS)
         {
-            const int e = e0 + lane;
+            const int off = a.offsets[e], count = a.counts[e];
             int       n = 0;
-            if(e < a.groups)
-            {
-                const int off = a.offsets[e], count = a.counts[e];
-                if(count > 0 && off >= 0 && off % MX4_BAND == 0 && count <= a.nq && off <= a.nq - count)
-                    n = (count + BN - 1) / BN;
-                else if(count != 0 && blockIdx.x == 0)
-                    atomicOr(&g_mx4_status, G_ERR_GROUP);
-            }
-            int up = n;
-#pragma unroll
-            for(int d = 1; d < 32; d <<= 1)
-            {
-                const int v = __shfl_up_sync(0xFFFFFFFFu, up, d);
-                if(lane >= d)
-                    up += v;
-            }
-            if(e < a.groups)
-                first_tile[e] = sum + up - n;
-            sum += __shfl_sync(0xFFFFFFFFu, up, 31);
+            if(count > 0 && off >= 0 && off % MX4_BAND == 0 && count <= a.nq && off <= a.nq - count)
+                n = (count + BN - 1) / BN;
+            else if(count != 0 && blockIdx.x == 0)
+                atomicOr(&g_mx4_status, G_ERR_GROUP);
+            first_tile[e] = n;
         }
-        if(lane == 0)
-            first_tile[a.groups] = sum;
+        __syncthreads();
+        if(warp == G_TMA_WARP)
+        {
+            int sum = 0;
+            for(int e0 = 0; e0 < a.groups; e0 += 32)
+            {
+                const int e = e0 + lane, n = e < a.groups ? first_tile[e] : 0;
+                int       up = n;
+#pragma unroll
+                for(int d = 1; d < 32; d <<= 1)
+                {
+                    const int v = __shfl_up_sync(0xFFFFFFFFu, up, d);
+                    if(lane >= d)
+                        up += v;
+                }
+                if(e < a.groups)
+                    first_tile[e] = sum + up - n;
+                sum += __shfl_sync(0xFFFFFFFFu, up, 31);
+            }
+            if(lane == 0)
+                first_tile[a.groups] = sum;
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -432,11 +473,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
     }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-
-    const int first = blockIdx.x / shared_by, stride = gridDim.x / shared_by;
-    const int total = (a.groups ? first_tile[a.groups] : (a.nq + BN - 1) / BN) * a.tiles_p;
-    const int part  = PAIR > 1 ? 0 : rank; // this CTA's range of K
-    const int kb0 = (int)((long long)a.kblocks * part / split), kb1 = (int)((long long)a.kblocks * (part + 1) / split);
+    const int      total     = (a.groups ? first_tile[a.groups] : (a.nq + BN - 1) / BN) * a.tiles_p;
     // the first wait of the CTA that gives up records where (bits 8..) and raises the abort flag for the others
     auto fail = [&](int where) {
         if(atomicExch(const_cast<int*>(abort_flag), 1) == 0)
@@ -449,27 +486,16 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
         // issues: with the loop inside `if(lane == 0)` the compiler moved every operand of every instruction to the uniform
         // registers as if lanes could differ, and the 8192 cube took 680 us instead of 285
         const bool issuer = elect_one();
-        uint32_t   s = 0, ph = 0;
+        uint32_t   s = filled % STAGES, ph = filled / STAGES;
         bool       ok = true;
         for(int tile = first; tile < total && ok; tile += stride)
         {
-            const Tile t    = tile_at<BN, L::TILE_P>(a, first_tile, tile);
-            const int  row  = t.group * a.np + t.p0 + lane0, q_row = t.q0 + (PAIR > 1 ? rank * L::Q_ROWS : 0);
-            const int  band = t.group * a.bands_p + (t.p0 + lane0) / MX4_BAND;
-            for(int kb = kb0; kb < kb1; ++kb)
+            const Tile t = tile_at<BN, L::TILE_P>(a, first_tile, tile);
+            for(int kb = kb0 + (tile == first ? filled : 0); kb < kb1; ++kb)
             {
                 if(!warp_wait(empty(s), ph ^ 1, abort_flag)) { fail(0); ok = false; break; }
                 if(issuer)
-                {
-                    const uint32_t st  = base + s * L::STAGE_BYTES;
-                    const uint32_t bar = PAIR > 1 ? cluster_addr(full(s), 0) : full(s);
-                    if(rank == 0 || PAIR == 1)
-                        mbar_arrive_expect_tx(full(s), PAIR * L::FILL_BYTES);
-                    load_codes<PAIR>(st, &maps.p, kb * G_ROW_BYTES, row, bar);
-                    load_codes<PAIR>(st + L::P_BYTES, &maps.q, kb * G_ROW_BYTES, q_row, bar);
-                    load_scales<PAIR>(st + L::P_BYTES + L::Q_BYTES, &maps.scales_p, kb * L::TILES, band, bar);
-                    load_scales<PAIR>(st + L::P_BYTES + L::Q_BYTES + L::P_SCALES, &maps.scales_q, kb * L::TILES, t.q0 / MX4_BAND, bar);
-                }
+                    fill(t, kb, s);
                 __syncwarp();
                 if(++s == STAGES)
                 {
@@ -494,7 +520,10 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
         bool       ok = true;
         for(int tile = first; tile < total && ok && (PAIR == 1 || rank == 0); tile += stride)
         {
-            const uint32_t q_col   = tile_at<BN, L::TILE_P>(a, first_tile, tile).q0 % MX4_BAND / 32; // columns of the scale tile before Q's rows
+            const Tile     t     = tile_at<BN, L::TILE_P>(a, first_tile, tile);
+            // Q's rows start at column q_col of the band's scales: 0, or 2 for the second tile of 64 (an odd column is a fault)
+            const uint32_t q_col = t.q0 % MX4_BAND / 32;
+            const uint32_t idesc = mx4_idesc<FMT, PAIR>(L::Q_BOX < L::Q_ROWS && t.q0 + L::Q_BOX >= t.q_end ? L::Q_BOX : BN);
             int            in_chunk = 0;
             for(int kb = kb0; kb < kb1; ++kb)
             {
@@ -526,7 +555,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                             constexpr int  per = FMT == B200_SGEMM_NVFP4 ? 1 : 2; // instructions per scale tile
                             const uint32_t id  = kk % per * 2;                    // first byte of the scale words it takes
                             constexpr int  off = G_KSTEP / 2 >> 4;
-                            tc_mma_mx4<FMT, PAIR>(d, dp + kk * off, dq + kk * off, mx4_idesc<FMT, BN, PAIR>() | id << 4 | id << 29,
+                            tc_mma_mx4<FMT, PAIR>(d, dp + kk * off, dq + kk * off, idesc | id << 4 | id << 29,
                                                   tp + kk / per * 4, tq + kk / per * 4 * L::Q_BANDS + q_col, in_chunk > 0 || kk > 0);
                         }
                     tc_commit<PAIR>(empty(s));
@@ -634,6 +663,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                     float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
                     for(int j = 0; j < COLS; ++j)
+                        if(t.q0 + q + j < t.q_end)
                         part[(q + j) * G_LANES + p] = acc[j];
                 }
             }
@@ -657,13 +687,15 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
             for(int j = threadIdx.x / G_LANES; j < mine; j += G_EPILOGUE / G_LANES)
             {
                 const int q = rank * mine + j;
+                if(t.q0 + q >= t.q_end)
+                    break;
                 float     sum[1] = {0.f};
                 for(int r = 0; r < split; ++r)
                 {
                     const float v = ld_cluster(base + (uint32_t)(q * G_LANES + p) * 4, r);
                     sum[0] = r == 0 ? v : sum[0] + v;
                 }
-                if(t.q0 + q < t.q_end && t.p0 + p < a.np)
+                if(t.p0 + p < a.np)
                 {
                     const long long at = (long long)(t.p0 + p) * a.sp + (long long)(t.q0 + q) * a.sq;
                     const float     v  = sum[0] * factor;
@@ -778,6 +810,15 @@ struct Operand
     size_t      rows, bands; // of the whole array: all groups
 };
 
+// CTAs that share a tile's K: more while the tiles leave half the SMs idle and each keeps four K blocks
+int split_of(unsigned long long tiles, int kblocks, int sms)
+{
+    int split = 1;
+    while(split < 8 && tiles * split * 2 <= (unsigned long long)sms && kblocks >= split * 2 * 4)
+        split *= 2;
+    return split;
+}
+
 template<int FMT, int BN, int PAIR>
 int launch(GArgs a, const Operand& p, const Operand& q, int sms, cudaStream_t stream)
 {
@@ -785,7 +826,7 @@ int launch(GArgs a, const Operand& p, const Operand& q, int sms, cudaStream_t st
     auto  kernel = mx4_gemm_kernel<FMT, BN, PAIR>;
     const size_t pitch = mx4_pitch((size_t)a.K), k_tiles = mx4_tiles(FMT, (size_t)a.K);
     Maps  maps;
-    if(!encode_codes(&maps.p, p.codes, p.rows, pitch, G_LANES) || !encode_codes(&maps.q, q.codes, q.rows, pitch, L::Q_ROWS)
+    if(!encode_codes(&maps.p, p.codes, p.rows, pitch, G_LANES) || !encode_codes(&maps.q, q.codes, q.rows, pitch, L::Q_BOX)
        || !encode_scales(&maps.scales_p, p.scales, k_tiles, p.bands, L::TILES, 1)
        || !encode_scales(&maps.scales_q, q.scales, k_tiles, q.bands, L::TILES, L::Q_BANDS))
         return B200_SGEMM_NO_KERNEL;
@@ -796,9 +837,7 @@ int launch(GArgs a, const Operand& p, const Operand& q, int sms, cudaStream_t st
     if(tiles > 0x7fffffffull)
         return B200_SGEMM_UNSUPPORTED_SIZE;
     // one tile per cluster where K is split, otherwise as many CTAs as there are tiles or SMs
-    a.split = 1;
-    while(PAIR == 1 && a.groups == 0 && a.split < 8 && tiles * a.split * 2 <= (unsigned long long)sms && a.kblocks >= a.split * 4)
-        a.split *= 2;
+    a.split = PAIR == 1 && a.groups == 0 ? split_of(tiles, a.kblocks, sms) : 1;
     const unsigned clusters = (unsigned)(a.split > 1 || tiles < (unsigned long long)(sms / PAIR) ? tiles : sms / PAIR);
     cudaError_t    e        = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM_BYTES);
     if(e != cudaSuccess)
@@ -823,8 +862,6 @@ int launch_tile(int bn, bool pair, const GArgs& a, const Operand& p, const Opera
 {
     if(pair)
         return bn == 256 ? launch<FMT, 256, 2>(a, p, q, sms, stream) : launch<FMT, 128, 2>(a, p, q, sms, stream);
-    if(bn == 32)
-        return launch<FMT, 32, 1>(a, p, q, sms, stream);
     if(bn == 64)
         return launch<FMT, 64, 1>(a, p, q, sms, stream);
     return launch<FMT, 128, 1>(a, p, q, sms, stream);
@@ -840,8 +877,13 @@ int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_
     a.kblocks = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
     a.chunk   = a.type == B200_SGEMM_F32 ? CHUNK_F32 : a.kblocks;
     a.bands_p = (a.np + MX4_BAND - 1) / MX4_BAND;
-    int  bn   = columns <= 32 ? 32 : (columns <= 64 ? 64 : 128);
+    int  bn   = columns <= 64 ? 64 : 128;
     bool pair = false;
+    // one product of few tiles: split K, and where K is too short for that halve the tiles as long as they fit on the SMs at once
+    // (1000 x 1030 x 515: 72 tiles of 128 columns 6.8 us, 144 of 64 see below)
+    auto tiles = [&](int n) { return ((unsigned long long)a.np + G_LANES - 1) / G_LANES * ((columns + n - 1) / n); };
+    if(a.groups == 0 && tiles(64) <= (unsigned long long)sms && split_of(tiles(128), a.kblocks, sms) == 1)
+        bn = 64;
     // pairs where they fill the SMs
     const size_t groups = a.groups ? a.groups : 1;
     const size_t pairs  = ((size_t)a.np + 255) / 256 * ((columns + 255) / 256) * groups;

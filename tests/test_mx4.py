@@ -373,7 +373,7 @@ def grouped_case(fmt, counts, N, K, rows=None, seed=0):
 @pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("counts,N,K", [([1], 1, 1), ([3, 0, 130, 1], 200, 300), ([0, 0, 5], 128, 256), ([33, 64, 20, 0, 300], 130, 1000),
-                                        ([1] * 40, 300, 2048), ([0, 0], 64, 64), ([500, 700], 520, 512), ([300, 0, 129, 700, 256, 1, 512, 400], 2200, 512)],
+                                        ([1] * 40, 300, 2048), ([0, 0], 64, 64), ([500, 700], 520, 512), ([40, 100, 1, 32, 64, 33, 65, 0, 0, 0, 0, 0, 0, 0, 0, 0], 130, 300), ([300, 0, 129, 700, 256, 1, 512, 400], 2200, 512)],
                          ids=lambda v: "-".join(map(str, v[:5])) if isinstance(v, list) else str(v))
 @pytest.mark.parametrize("hint", [0, 1])
 def test_grouped(sgemm, fmt, dtype, counts, N, K, hint):
