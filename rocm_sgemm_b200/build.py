@@ -112,7 +112,8 @@ def build_library(config: Path | None = None, jobs: int | None = None, verbose=F
                  kernel_hdr + [CSRC / "tcgen05.cuh", CSRC / "transpose.hpp", REPO / "include" / "b200_sgemm.h"]))
     mx4_deps = [CSRC / "mx4_common.cuh", REPO / "include" / "b200_sgemm.h"]
     work.append((CSRC / "mx4_quantize.cu", mx4_deps))
-    work.append((CSRC / "mx4_gemm.cu", mx4_deps + kernel_hdr + [CSRC / "tcgen05.cuh"]))
+    work.append((CSRC / "mx4_few.cu", mx4_deps + [CSRC / "mx4_few.hpp"]))
+    work.append((CSRC / "mx4_gemm.cu", mx4_deps + [CSRC / "mx4_few.hpp"] + kernel_hdr + [CSRC / "tcgen05.cuh"]))
     work.append((CSRC / "route.cu", mx4_deps))
     work.append((CSRC / "sgemm_blas.cu", [REPO / "include" / "b200_sgemm.h"]))
     work.append((CSRC / "sgemm_selftest.cu", kernel_hdr + [REPO / "include" / "b200_sgemm.h"]))

@@ -85,6 +85,18 @@ __device__ __forceinline__ float e4m3_value(unsigned byte) { return __uint_as_fl
 // value of an e8m0 byte below 0xFF: 2^(byte - 127)
 __device__ __forceinline__ float e8m0_value(unsigned byte) { return byte ? __uint_as_float(byte << 23) : __uint_as_float(1u << 22); }
 
+constexpr unsigned NAN_E4M3 = 0x7Fu;
+constexpr unsigned NAN_E8M0 = 0xFFu;
+// the value of a scale byte
+template<int FMT>
+__device__ __forceinline__ float scale_value(unsigned byte)
+{
+    const float nan = __uint_as_float(0x7FC00000u);
+    if(FMT == B200_SGEMM_NVFP4)
+        return (byte & 0x7Fu) == NAN_E4M3 ? nan : e4m3_value(byte);
+    return byte == NAN_E8M0 ? nan : e8m0_value(byte);
+}
+
 // f(type as a C++ type) for a checked element type
 template<class F>
 int with_type(int type, F f)

@@ -1,0 +1,31 @@
+// The 4-bit product for a few rows on one side (mx4_few.cu).
+#pragma once
+#include <cstddef>
+#include <cuda_runtime.h>
+
+namespace sgemm_b200
+{
+// whether mx4_few takes the product: one row, or two against a matrix of which they cost less than the tensor core's set-up
+// (measured: two rows x 4096 x 4096 6.1 us against 7.4, x 16384 x 4096 17 us against 11; one row 4.6 against 7.3, 11.2 against 10.9)
+inline bool mx4_is_few(size_t few, size_t rows, size_t K)
+{
+    return few == 1 ? rows * K <= (size_t(1) << 26) : few == 2 && rows * K <= (size_t(1) << 24);
+}
+
+struct FewArgs
+{
+    const void*  codes;  // the long side: `rows` rows
+    const void*  scales;
+    const void*  codes_x; // the short side: `few` rows
+    const void*  scales_x;
+    const float* global;
+    const float* global_x;
+    void*        c;
+    long long    ld_long, ld_few; // element strides of C along the two sides
+    float        alpha;
+    int          rows, few, K, type;
+};
+
+// status as b200_sgemm_mx4's
+int mx4_few(int format, const FewArgs& a, int sms, cudaStream_t stream);
+} // namespace sgemm_b200

@@ -28,6 +28,7 @@
 // workspace is needed (a captured graph can be replayed on any stream).
 // Every wait is bounded, as in the other kernels.
 #include "mx4_common.cuh"
+#include "mx4_few.hpp"
 #include "sgemm_ws_kernel.cuh"
 #include "tcgen05.cuh"
 
@@ -917,6 +918,29 @@ extern "C" int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, con
     if(ldc > (size_t(1) << 40))
         return B200_SGEMM_UNSUPPORTED_SIZE;
     const Operand a{a_codes, a_scales, M, (M + MX4_BAND - 1) / MX4_BAND}, b{b_codes, b_scales, N, (N + MX4_BAND - 1) / MX4_BAND};
+    if(mx4_is_few(M < N ? M : N, M < N ? N : M, K))
+    {
+        const bool b_long = N >= M;
+        int        sms = 0, status = device_sms(&sms);
+        if(status != B200_SGEMM_OK)
+            return status;
+        FewArgs f;
+        f.codes    = b_long ? b_codes : a_codes;
+        f.scales   = b_long ? b_scales : a_scales;
+        f.codes_x  = b_long ? a_codes : b_codes;
+        f.scales_x = b_long ? a_scales : b_scales;
+        f.global   = b_long ? global_b : global_a;
+        f.global_x = b_long ? global_a : global_b;
+        f.c        = C;
+        f.ld_long  = b_long == row ? 1 : (long long)ldc;
+        f.ld_few   = b_long == row ? (long long)ldc : 1;
+        f.alpha    = alpha;
+        f.rows     = (int)(b_long ? N : M);
+        f.few      = (int)(b_long ? M : N);
+        f.K        = (int)K;
+        f.type     = type_c;
+        return mx4_few(format, f, sms, static_cast<cudaStream_t>(cuda_stream));
+    }
     // lanes: C's contiguous dimension, unless that one is short and the other is not
     bool b_lanes = row;
     if(packed <= 64 && (row ? M : N) > packed)

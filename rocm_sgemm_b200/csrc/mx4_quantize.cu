@@ -34,8 +34,6 @@ static_assert(Q_ROWS == 32, "the rows of a CTA lie 16 bytes apart in a scale til
 constexpr int Q_COL_K   = 128;           // k of one CTA when the rows are the contiguous dimension
 
 constexpr unsigned INF_BITS  = 0x7F800000u;
-constexpr unsigned NAN_E4M3  = 0x7Fu;
-constexpr unsigned NAN_E8M0  = 0xFFu;
 
 // the matrix's scale, as every thread needs it
 struct Global
@@ -416,16 +414,6 @@ __device__ __forceinline__ float2 levels2(unsigned byte)
     const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1);
     return __half22float2(__half2(h));
 }
-// the value of a scale byte
-template<int FMT>
-__device__ __forceinline__ float scale_value(unsigned byte)
-{
-    const float nan = __uint_as_float(0x7FC00000u);
-    if(FMT == B200_SGEMM_NVFP4)
-        return (byte & 0x7Fu) == NAN_E4M3 ? nan : e4m3_value(byte);
-    return byte == NAN_E8M0 ? nan : e8m0_value(byte);
-}
-
 // One CTA: 32 rows x 512 k, a warp four rows.  A lane turns 32 bytes of output at a time, with the codes and scales of all four
 // rows in flight at once.
 template<int FMT, class T>

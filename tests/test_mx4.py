@@ -265,7 +265,7 @@ def check(got, want, bound):
 
 
 SHAPES = [(1, 1, 1), (1, 128, 64), (3, 5, 7), (128, 128, 256), (17, 130, 100), (33, 257, 515), (65, 64, 320), (129, 300, 1000),
-          (200, 520, 2048), (1, 700, 4096), (20, 256, 8192), (300, 2, 777), (1000, 16, 200), (512, 640, 130)]
+          (200, 520, 2048), (1, 700, 4096), (20, 256, 8192), (300, 2, 777), (4, 129, 2048), (3, 1000, 5000), (2100, 1, 96), (2, 4, 33), (4, 4, 640), (5, 300, 4096), (1000, 16, 200), (512, 640, 130)]
 
 
 @gpu
