@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(F_THREADS) mx4_few_kernel(const __grid_constan
         fetch(k + step);
         const size_t at = (size_t)(k / BLOCK / 4) * MX4_TILE_BYTES;
         const int    in = k / BLOCK % 4 * 8;
-        float   sx[FEW][BLOCKS]; // of the short side, and what raw_scale of the long side lacks
+        float   sx[FEW][BLOCKS]; // of the short side, times 2^100 of the 2^120 that raw_scale lacks (448 x 2^120 is no FP32 number)
         __half2 v[FEW][2][8];
 #pragma unroll
         for(int m = 0; m < FEW; ++m)
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(F_THREADS) mx4_few_kernel(const __grid_constan
             const unsigned s = __ldg(reinterpret_cast<const unsigned*>(scales_x + at + m * 16)) >> in;
 #pragma unroll
             for(int b = 0; b < BLOCKS; ++b)
-                sx[m][b] = scale_value<FMT>(s >> (8 * b) & 0xFFu) * (FMT == B200_SGEMM_NVFP4 ? 0x1p120f : 1.f);
+                sx[m][b] = scale_value<FMT>(s >> (8 * b) & 0xFFu) * (FMT == B200_SGEMM_NVFP4 ? 0x1p100f : 1.f);
             pairs16(v[m][0], x.x, x.y);
             pairs16(v[m][1], x.z, x.w);
         }
@@ -169,6 +169,8 @@ __global__ void __launch_bounds__(F_THREADS) mx4_few_kernel(const __grid_constan
         total += part[warp + i][lane];
     if(q >= rows)
         return;
+    if(FMT == B200_SGEMM_NVFP4)
+        total *= 0x1p20f;
     float factor = a.f.alpha;
     if(a.f.global_x)
         factor *= *a.f.global_x;

@@ -295,6 +295,32 @@ def test_product(sgemm, fmt, layout_c, dtype, shape):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N", [(1, 300), (2, 129), (40, 130), (200, 1), (300, 200), (2100, 2300)])
+def test_product_over_the_whole_range_of_scales(sgemm, fmt, dtype, M, N):
+    """The smallest and the largest scales of both formats, zero scales among them; products stay in FP32's range."""
+    K = 1100
+    r = np.random.default_rng(M)
+    sides = []
+    for rows, sign in ((M, 1), (N, -1)):
+        code = r.integers(0, 16, (rows, K)).astype(np.uint8)
+        blocks = -(-K // ref.BLOCK[fmt])
+        if fmt == ref.NVFP4:
+            byte = r.choice([0, 1, 7, 8, 0x38, 0x70, 0x7D, 0x7E], (rows, blocks))
+        else:  # 2^+-100 on one side against 2^-+100 on the other, and 2^-127
+            byte = np.where(r.random((rows, blocks)) < 0.1, 0, 127 + sign * 100 + r.integers(-12, 12, (rows, blocks)))
+        byte = byte.astype(np.uint8)
+        sides.append((*(dev(v) for v in ref.pack(fmt, code, byte)), ref.values(fmt, code, byte)))
+    a, b = sides
+    c = torch.empty(M, N, dtype=TYPES[dtype], device="cuda")
+    sgemm.gemm_mx4(fmt, 0, pkg.m_type[dtype], c, a[0], a[1], b[0], b[1], M, N, K)
+    want = a[2] @ b[2].T
+    check(c, want, ref.product_bound(a[2], b[2], want, dtype))
+    assert sgemm.mx4_device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_product_many_tiles(sgemm, fmt, dtype):
     """More tiles than SMs, packed C, and the same bits on every call."""
     M, N, K = 1500, 2200, 1100
