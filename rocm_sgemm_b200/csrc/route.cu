@@ -502,9 +502,12 @@ extern "C" int b200_sgemm_route_sort(const int* expert_ids, size_t tokens, size_
     a.warps           = per_cta >= SORT_THREADS ? SORT_WARPS : (per_cta + 31) / 32;
     a.per_warp        = ((per_cta + a.warps - 1) / a.warps + 31) / 32 * 32;
     const size_t smem = (size_t)a.warps * experts * sizeof(int);
-    cudaError_t  e    = cudaFuncSetAttribute(route_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if(e != cudaSuccess)
-        return (int)e;
+    if(smem > 48 * 1024 - sizeof(int) * (2 * MAX_EXPERTS + SORT_WARPS)) // beyond what every kernel may have
+    {
+        const cudaError_t e = cudaFuncSetAttribute(route_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if(e != cudaSuccess)
+            return (int)e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3((unsigned)a.ctas);
     cfg.blockDim           = dim3(SORT_THREADS);
