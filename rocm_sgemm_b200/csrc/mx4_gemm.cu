@@ -9,23 +9,24 @@
 //            that is the weights, and the tokens cost 32 or 64 columns instead of a tile of 128 rows
 //   columns  the other one; the rows of the groups in the grouped product
 //
-// Tiles.  128 lanes x 64 or 128 columns by one CTA, or 256 lanes x 128 or 256 columns by a pair of CTAs on
-// neighbouring SMs: each holds 128 of the lanes, half of Q's rows and all of Q's scales, and the first one issues for both.
-// A pair reads half of Q from the L2 and from shared memory and issues half the scale copies per product.
+// Tiles.  128 lanes x 64 or 128 columns by one CTA, or 256 lanes x 256 columns by a pair of CTAs on neighbouring SMs: each holds
+// 128 of the lanes, half of Q's rows and all of Q's scales, and the first one issues for both.  A pair reads half of Q from the
+// L2 and from shared memory and issues half the scale copies per product.
 //
 // One persistent CTA per SM, 10 warps:
 //   warps 0-7  accumulate and store.  The tensor core adds into its FP32 accumulator with truncation, so for an FP32
-//              result the accumulator is emptied into registers every CHUNK_F32 K blocks and the parts are added there,
-//              rounded to nearest; results of 16 bits keep one accumulator for the whole of K (a bias of at most 2^-23 a
-//              product of 64 k is below their rounding up to K = 2^18).
+//              result the accumulator is emptied into registers every 1024 or 2048 k and the parts are added there,
+//              rounded to nearest (relative error of the whole result with operands of a wide range, K = 16384: 1.2e-7 in parts
+//              of 256 k, 2.9e-7 of 1024, 5.3e-7 of 2048; an FP32 product on the FMA pipe 2.4e-7); results of 16 bits keep one
+//              accumulator for the whole of K (a bias of at most 2^-23 a product of 64 k, below their rounding up to K = 2^18).
 //   warp 8     fetches the stages by TMA: the two operands' codes (256 k = rows of 128 bytes, 128-byte swizzle) and the scale
 //              tiles as they lie; zero beyond the matrix
 //   warp 9     copies the stage's scale tiles into tensor memory (tcgen05.cp, replicated to the four lane quarters) and issues
 //              the products, 64 k each.  Scales go to a tensor-memory slot of the stage's own, which is free as soon as the
 //              stage is.
-// Few tiles: a cluster of 2, 4 or 8 CTAs shares a tile, each with a range of K of its own; the parts meet through
-// distributed shared memory and are added in ascending order of K, so the result does not depend on timing and no
-// workspace is needed (a captured graph can be replayed on any stream).
+// Few tiles: a cluster of 2, 4 or 8 CTAs shares a tile, each with a range of K of its own; every CTA sends its part of a column
+// to the one that will store it, from shared memory to shared memory, which adds the parts in ascending order of K, so the
+// result does not depend on timing and no workspace is needed (a captured graph can be replayed on any stream).
 // Every wait is bounded, as in the other kernels.
 #include "mx4_common.cuh"
 #include "mx4_few.hpp"
@@ -47,11 +48,16 @@ constexpr int G_KSTEP      = 64; // k of one instruction
 constexpr int G_EPILOGUE   = 256;
 constexpr int G_TMA_WARP   = 8;
 constexpr int G_MMA_WARP   = 9;
-constexpr int G_THREADS    = 320;
 constexpr int G_TMEM_COLS  = 512;
 constexpr int G_SCALE_COL  = 256; // tensor-memory columns 0..255: accumulators; behind them a slot of scales per stage
 constexpr int G_MAX_GROUPS = 1024;
+constexpr int MAX_SPLIT    = 8; // CTAs that share a tile's K
 constexpr int CHUNK_F32    = 4; // K blocks (1024 k, 16 products) added inside the tensor core for an FP32 result
+constexpr int CHUNK_F32_WIDE = 8; // the same for 256 columns, whose one accumulator stands still while it is emptied
+// Registers of the kernel that keeps 128 FP32 sums a thread: 12 warps are launched with 168 each; warps 8 to 11 give theirs up
+// and warps 0 to 7 take them: 256 x 224 + 128 x 56 = 384 x 168, exactly the launch's allocation, so the increase is always granted.
+constexpr int G_LAUNCH_REGS = 168, G_SUM_REGS = 224, G_ISSUE_REGS = 56;
+static_assert(G_EPILOGUE * G_SUM_REGS + 128 * G_ISSUE_REGS == (G_EPILOGUE + 128) * G_LAUNCH_REGS, "register budgets");
 
 constexpr int G_ERR_WAIT  = 1; // status bits: a wait gave up (bits 8.. say which);
 constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the matrix, the group was left out
@@ -59,9 +65,11 @@ constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the mat
 __device__ int g_mx4_status;
 
 // PAIR: CTAs that share a tile's instructions
-template<int FMT, int BN, int PAIR>
+// SUMS: 256 columns of FP32 results, added in registers
+template<int FMT, int BN, int PAIR, bool SUMS = false>
 struct GLayout
 {
+    static constexpr int    THREADS     = SUMS ? G_EPILOGUE + 128 : G_EPILOGUE + 64;
     static constexpr int    TILE_P      = PAIR * G_LANES;
     static constexpr int    Q_ROWS      = BN / PAIR;                     // of this CTA
     static constexpr int    Q_BOX       = BN == 64 ? 32 : Q_ROWS;        // rows of one copy; a tile of up to 32 rows takes one of two
@@ -78,13 +86,14 @@ struct GLayout
     static constexpr int    BY_TMEM     = (G_TMEM_COLS - G_SCALE_COL) / SLOT_COLS;
     static constexpr int    STAGES      = BY_SMEM < BY_TMEM ? (BY_SMEM < 8 ? BY_SMEM : 8) : (BY_TMEM < 8 ? BY_TMEM : 8);
     static constexpr int    ACCS        = BN > 128 ? 1 : 2; // accumulators
-    static constexpr int    BARRIERS    = 2 * STAGES + 5;
+    static constexpr int    BARRIERS    = 2 * STAGES + 6;
     static constexpr size_t SMEM_BYTES  = size_t(STAGES) * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers, misc*/;
     static_assert(8 * BARRIERS + 16 <= 256, "barrier area");
     static_assert(ACCS * BN <= G_SCALE_COL, "tensor memory");
     static_assert(BN % 64 == 0 && SLOT_COLS % 4 == 0 && TILES % 2 == 0, "scales start on an even column");
     static_assert(SMEM_BYTES + (G_MAX_GROUPS + 1) * 4 <= 227 * 1024, "shared memory");
-    static_assert(PAIR > 1 || BN * G_LANES * 4 <= STAGES * STAGE_BYTES, "the parts of a split tile lie in the ring");
+    static_assert(PAIR > 1 || (BN + MAX_SPLIT) * G_LANES * 4 <= STAGES * STAGE_BYTES / 2, "a split tile's parts lie in the ring twice");
+    static_assert(PAIR > 1 || STAGES * STAGE_BYTES / 2 % 16 == 0, "bulk copies start on 16 bytes");
 };
 
 struct GArgs
@@ -188,11 +197,12 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
     return at;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank)
+// this CTA's shared memory to another's, whose barrier counts the bytes
+__device__ __forceinline__ void bulk_send(uint32_t cluster_dst, uint32_t src, uint32_t bytes, uint32_t cluster_bar)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(addr, rank)) : "memory");
-    return v;
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(cluster_dst), "r"(src), "r"(bytes), "r"(cluster_bar)
+                 : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
 {
@@ -318,6 +328,15 @@ struct Maps<1>
     CUtensorMap p, q;
 };
 
+// the first n of N results, `stride` elements apart
+template<class T, int N>
+__device__ __forceinline__ void store_strided(T* c, const float (&v)[N], float factor, long long stride, int n)
+{
+#pragma unroll
+    for(int j = 0; j < N; ++j)
+        if(j < n)
+            c[j * stride] = from_float<T>(v[j] * factor);
+}
 // two results of 16 bits as they are stored, the first in the lower half
 __device__ __forceinline__ uint32_t pack16(int type, float x, float y)
 {
@@ -361,10 +380,10 @@ __device__ __forceinline__ void store_packed(const GArgs& a, const uint32_t (&v)
     }
 }
 
-template<int FMT, int BN, int PAIR>
-__global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ Maps<PAIR> maps)
+template<int FMT, int BN, int PAIR, bool SUMS>
+__global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ Maps<PAIR> maps)
 {
-    using L = GLayout<FMT, BN, PAIR>;
+    using L = GLayout<FMT, BN, PAIR, SUMS>;
     constexpr int STAGES = L::STAGES;
     constexpr int COLS   = BN / 2; // columns of one epilogue thread
     extern __shared__ uint8_t smem_raw[];
@@ -377,7 +396,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
     auto empty     = [&](int s) { return bar_base + 8u * (STAGES + s); };
     auto acc_full  = [&](int b) { return bar_base + 8u * (2 * STAGES + b); };
     auto acc_empty = [&](int b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
-    const uint32_t drained = bar_base + 8u * (2 * STAGES + 4);
+    const uint32_t drained = bar_base + 8u * (2 * STAGES + 4), parts = drained + 8u;
     uint8_t*       misc       = ring + STAGES * L::STAGE_BYTES + 8 * L::BARRIERS;
     uint32_t*      tmem_slot  = reinterpret_cast<uint32_t*>(misc);
     volatile int*  abort_flag = reinterpret_cast<volatile int*>(misc + 8);
@@ -433,6 +452,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                 mbar_init(acc_empty(b), PAIR * G_EPILOGUE / 32);
             }
             mbar_init(drained, 1);
+            mbar_init(parts, 1);
             *abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -455,7 +475,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
     }
     if(a.groups) // column tiles before each group
     {
-        for(int e = threadIdx.x; e < a.groups; e += G_THREADS)
+        for(int e = threadIdx.x; e < a.groups; e += L::THREADS)
         {
             const int off = a.offsets[e], count = a.counts[e];
             int       n = 0;
@@ -504,6 +524,8 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
             atomicOr(&g_mx4_status, G_ERR_WAIT | (256 << where));
     };
 
+    if(SUMS && warp >= G_EPILOGUE / 32) // the whole warpgroup 8 to 11
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G_ISSUE_REGS));
     if(warp == G_TMA_WARP)
     {
         // here and below the whole warp walks the loop, so that addresses and descriptors are uniform, and one thread
@@ -606,8 +628,10 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
             drain_wait(drained, 0);
         }
     }
-    else
+    else if(warp < G_EPILOGUE / 32)
     {
+        if constexpr(SUMS)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G_SUM_REGS));
         const int quarter = warp & 3, half = warp >> 2;
         uint32_t  buf = 0, acc_ph = 0;
         bool      ok     = true;
@@ -618,9 +642,9 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
         for(int tile = first; tile < total && ok; tile += stride)
         {
             const Tile t = tile_at<BN, L::TILE_P>(a, first_tile, tile);
-            if constexpr(L::ACCS == 1) // results of 16 bits: rounded into registers, so that the one accumulator is free at once
+            const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q; // fetched while the tile is computed
+            if constexpr(L::ACCS == 1 && !SUMS) // results of 16 bits: rounded into registers, so that the one accumulator is free at once
             {
-                const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q;
                 uint32_t    out[COLS / 2];
                 if(!warp_wait(acc_full(0), acc_ph, abort_flag)) { fail(3); ok = false; break; }
                 tc_fence_after();
@@ -651,23 +675,40 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                     if(!warp_wait(acc_full(buf), acc_ph, abort_flag)) { fail(3); ok = false; break; }
                     tc_fence_after();
                     const uint32_t from = tmem_base + buf * BN + half * COLS + (uint32_t(quarter * 32) << 16);
-                    uint32_t v[COLS];
+                    // SUMS: 16 columns at a time, added while the next are on their way (32 at a time spill)
+                    constexpr int STEP = SUMS ? 16 : COLS;
+                    uint32_t      v[2][STEP];
+                    auto          load = [&](int c) {
 #pragma unroll
-                    for(int j = 0; j < COLS; j += 16)
-                        tmem_ld16(from + j, v + j);
-                    tmem_ld_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if(lane == 0) // the accumulator is free before its values are added
+                        for(int j = 0; j < STEP; j += 16)
+                            tmem_ld16(from + c + j, v[c / STEP % 2] + j);
+                    };
+                    load(0);
+#pragma unroll
+                    for(int c = 0; c < COLS; c += STEP)
                     {
-                        if(PAIR > 1)
-                            mbar_arrive_cluster(cluster_addr(acc_empty(buf), 0));
+                        tmem_ld_wait();
+                        if(c + STEP < COLS)
+                            load(c + STEP);
                         else
-                            mbar_arrive(acc_empty(buf));
-                    }
+                        {
+                            tc_fence_before();
+                            __syncwarp();
+                            if(lane == 0) // the accumulator is free before its last values are added
+                            {
+                                if(PAIR > 1)
+                                    mbar_arrive_cluster(cluster_addr(acc_empty(buf), 0));
+                                else
+                                    mbar_arrive(acc_empty(buf));
+                            }
+                        }
 #pragma unroll
-                    for(int j = 0; j < COLS; ++j)
-                        acc[j] = ch == 0 ? __uint_as_float(v[j]) : acc[j] + __uint_as_float(v[j]);
+                        for(int j = 0; j < STEP; ++j)
+                        {
+                            const float part = __uint_as_float(v[c / STEP % 2][j]);
+                            acc[c + j]       = ch == 0 ? part : acc[c + j] + part;
+                        }
+                    }
                     if(++buf == L::ACCS)
                     {
                         buf = 0;
@@ -679,16 +720,19 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
                 const int p = lane0 + quarter * 32 + lane, q = half * COLS;
                 if(PAIR > 1 || split == 1)
                 {
-                    const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q;
-                    store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
+                    if constexpr(SUMS)
+                        store_columns<float>(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
+                    else
+                        store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
                 }
-                else // park the part; a cluster has one tile, so the ring is at rest
+                else // park the part in the ring, which is at rest: a CTA of a split tile has no other
                 {
-                    float* part = reinterpret_cast<float*>(ring);
+                    float* parked = reinterpret_cast<float*>(ring);
 #pragma unroll
                     for(int j = 0; j < COLS; ++j)
                         if(t.q0 + q + j < t.q_end)
-                        part[(q + j) * G_LANES + p] = acc[j];
+                            parked[(q + j) * G_LANES + p] = acc[j];
+                    fence_async_smem(); // for the copies below
                 }
             }
         }
@@ -697,41 +741,66 @@ __global__ void __launch_bounds__(G_THREADS, 1) mx4_gemm_kernel(const __grid_con
     __syncwarp();
     if(PAIR == 1 && split > 1)
     {
-        cluster_arrive();
+        cluster_arrive(); // all parts are parked and all rings at rest
         cluster_wait();
-        if(first < total && warp < G_EPILOGUE / 32) // rank r adds and stores columns r * BN / split ..
+        if(first < total && warp < G_EPILOGUE / 32)
         {
-            const Tile  t      = tile_at<BN, L::TILE_P>(a, first_tile, first);
-            float       factor = a.alpha;
-            if(a.global_q)
-                factor *= *a.global_q;
-            if(a.global_p)
-                factor *= a.global_p[t.group];
-            const int p = threadIdx.x & (G_LANES - 1), mine = BN / split;
-            for(int j = threadIdx.x / G_LANES; j < mine; j += G_EPILOGUE / G_LANES)
+            // CTA r adds and stores columns r * share .. of the tile; the others' parts come by bulk copies into the upper half of
+            // its ring (single words written or read across the cluster take about 60 cycles a warp: 6 us for 64 columns)
+            constexpr uint32_t UPPER = STAGES * L::STAGE_BYTES / 2;
+            const Tile         t       = tile_at<BN, L::TILE_P>(a, first_tile, first);
+            const int          columns = min(BN, t.q_end - t.q0), share = (columns + split - 1) / split;
+            const int          mine    = max(0, min(share, columns - rank * share));
+            if(threadIdx.x == 0 && mine)
+                mbar_arrive_expect_tx(parts, (uint32_t)(split - 1) * mine * G_LANES * 4);
+            if(threadIdx.x < split && threadIdx.x != rank)
             {
-                const int q = rank * mine + j;
-                if(t.q0 + q >= t.q_end)
-                    break;
-                float     sum[1] = {0.f};
-                for(int r = 0; r < split; ++r)
+                const int r = threadIdx.x, theirs = max(0, min(share, columns - r * share));
+                if(theirs)
+                    bulk_send(cluster_addr(base + UPPER + (uint32_t)(rank * share * G_LANES) * 4, r), base + (uint32_t)(r * share * G_LANES) * 4,
+                              (uint32_t)theirs * G_LANES * 4, cluster_addr(parts, r));
+            }
+            __syncwarp();
+            if(mine && !warp_wait(parts, 0, abort_flag))
+                fail(4);
+            else
+            {
+                float factor = a.alpha;
+                if(a.global_q)
+                    factor *= *a.global_q;
+                if(a.global_p)
+                    factor *= a.global_p[t.group];
+                const float* own   = reinterpret_cast<const float*>(ring) + rank * share * G_LANES;
+                const float* other = reinterpret_cast<const float*>(ring + UPPER); // [rank][column][lane]
+                const int    p     = threadIdx.x & (G_LANES - 1);
+                // eight columns at a time, so that their reads overlap
+                constexpr int STEP = 8, STRIDE = G_EPILOGUE / G_LANES;
+                for(int i0 = threadIdx.x / G_LANES; i0 < mine; i0 += STEP * STRIDE)
                 {
-                    const float v = ld_cluster(base + (uint32_t)(q * G_LANES + p) * 4, r);
-                    sum[0] = r == 0 ? v : sum[0] + v;
-                }
-                if(t.p0 + p < a.np)
-                {
-                    const long long at = (long long)(t.p0 + p) * a.sp + (long long)(t.q0 + q) * a.sq;
-                    const float     v  = sum[0] * factor;
+                    float sum[STEP];
+#pragma unroll
+                    for(int j = 0; j < STEP; ++j)
+                        sum[j] = 0.f;
+                    for(int r = 0; r < split; ++r)
+                    {
+                        const float* from = r == rank ? own : other + r * share * G_LANES;
+#pragma unroll
+                        for(int j = 0; j < STEP; ++j)
+                            if(i0 + j * STRIDE < mine)
+                                sum[j] += from[(i0 + j * STRIDE) * G_LANES + p];
+                    }
+                    const long long at = (long long)(t.p0 + p) * a.sp + (long long)(t.q0 + rank * share + i0) * a.sq;
+                    const int       n  = t.p0 + p < a.np ? (mine - i0 + STRIDE - 1) / STRIDE : 0;
                     if(a.type == B200_SGEMM_F32)
-                        static_cast<float*>(a.c)[at] = v;
+                        store_strided(static_cast<float*>(a.c) + at, sum, factor, STRIDE * a.sq, n);
                     else if(a.type == B200_SGEMM_F16)
-                        static_cast<__half*>(a.c)[at] = from_float<__half>(v);
+                        store_strided(static_cast<__half*>(a.c) + at, sum, factor, STRIDE * a.sq, n);
                     else
-                        static_cast<__nv_bfloat16*>(a.c)[at] = from_float<__nv_bfloat16>(v);
+                        store_strided(static_cast<__nv_bfloat16*>(a.c) + at, sum, factor, STRIDE * a.sq, n);
                 }
             }
         }
+        __syncwarp();
         cluster_arrive(); // nobody leaves while its part is being read
         cluster_wait();
     }
@@ -835,20 +904,52 @@ struct Operand
     size_t      rows, bands; // of the whole array: all groups
 };
 
-// CTAs that share a tile's K: more while the tiles leave half the SMs idle and each keeps four K blocks
-int split_of(unsigned long long tiles, int kblocks, int sms)
+// How a product is cut: the columns of a tile (256: by pairs of CTAs) and the CTAs that share its K.
+struct Cut
 {
-    int split = 1;
-    while(split < 8 && tiles * split * 2 <= (unsigned long long)sms && kblocks >= split * 2 * 4)
-        split *= 2;
-    return split;
+    int columns, split;
+};
+// The cut with the least estimated time, from what a few dozen shapes between 100 x 1000 x 300 and 2560^3 measured (us, BF16
+// result): a K block takes 0.33 / 0.37 / 0.37 in tiles of 64 / 128 / 256 columns, for the SMs go through it at about the same pace
+// whatever its width; storing a tile 1.3 / 2.4 / 2.5 where the next tile's blocks do not hide it, and 0.5 / 1 / 2 more at the end;
+// adding the parts of a split tile 1.4 / 2.4 for 64 / 128 columns.  Examples, us for (columns, split): 2048^3 (128, 1) 12.6,
+// (256, 1) 9.8; 128 x 8192 x 8192 (64, 1) 15.3, (128, 2) 14.5, (256, 1) 16.3; 512 x 512 x 8192 (64, 1) 14.2, (64, 4) 10.1;
+// 512^3 (64, 1) 5.8, (64, 2) 7.2, (128, 1) 6.7.
+// lane_rows, column_rows: extents of one group; clusters of 8 and 4 CTAs do not fill every part of the chip, so they are held
+// below three quarters and seven eighths of the SMs.
+Cut cut_of(size_t lane_rows, size_t column_rows, size_t groups, int kblocks, bool may_split, int sms)
+{
+    Cut   best = {64, 1};
+    float least = 1e30f;
+    for(int i = 0; i < 3; ++i)
+    {
+        const int    columns = 64 << i, lanes = i == 2 ? 256 : 128, slots = i == 2 ? sms / 2 : sms;
+        const float  block = i == 0 ? 0.33f : 0.37f, store = i == 0 ? 1.3f : (i == 1 ? 2.4f : 2.5f);
+        const float  end = i == 0 ? 0.5f : (i == 1 ? 1.f : 2.f), join = i == 0 ? 1.4f : 2.4f;
+        const size_t tiles = (lane_rows + lanes - 1) / lanes * ((column_rows + columns - 1) / columns) * groups;
+        for(int split = 1; split <= (may_split && i < 2 ? MAX_SPLIT : 1); split *= 2)
+        {
+            const size_t room = split == 8 ? sms * 3 / 4 : (split == 4 ? sms * 7 / 8 : slots);
+            if(split > 1 && (tiles * split > room || split > kblocks))
+                break;
+            const float waves = (float)((tiles * split + slots - 1) / slots);
+            const float one   = (float)((kblocks + split - 1) / split) * block;
+            const float time  = (waves - 1.f) * (one > store ? one : store) + one + end + (split > 1 ? join : 0.f);
+            if(time < least)
+            {
+                least = time;
+                best  = {columns, split};
+            }
+        }
+    }
+    return best;
 }
 
-template<int FMT, int BN, int PAIR>
+template<int FMT, int BN, int PAIR, bool SUMS = false>
 int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cudaStream_t stream)
 {
-    using L      = GLayout<FMT, BN, PAIR>;
-    auto  kernel = mx4_gemm_kernel<FMT, BN, PAIR>;
+    using L      = GLayout<FMT, BN, PAIR, SUMS>;
+    auto  kernel = mx4_gemm_kernel<FMT, BN, PAIR, SUMS>;
     const size_t pitch = mx4_pitch((size_t)a.K), k_tiles = mx4_tiles(FMT, (size_t)a.K);
     Maps<PAIR> maps;
     if(!encode_codes(&maps.p, p.codes, p.rows, pitch, G_LANES) || !encode_codes(&maps.q, q.codes, q.rows, pitch, L::Q_BOX))
@@ -869,7 +970,6 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
     if(tiles > 0x7fffffffull)
         return B200_SGEMM_UNSUPPORTED_SIZE;
     // one tile per cluster where K is split, otherwise as many CTAs as there are tiles or SMs
-    a.split = PAIR == 1 && a.groups == 0 ? split_of(tiles, a.kblocks, sms) : 1;
     const unsigned clusters = (unsigned)(a.split > 1 || tiles < (unsigned long long)(sms / PAIR) ? tiles : sms / PAIR);
     static std::atomic<unsigned long long> ready{0}; // devices on which the kernel may have its shared memory
     const unsigned long long               bit = 1ull << (device % MAX_DEVICES);
@@ -878,11 +978,19 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM_BYTES);
         if(e != cudaSuccess)
             return (int)e;
+        if(SUMS)
+        {
+            cudaFuncAttributes f;
+            if(const cudaError_t e = cudaFuncGetAttributes(&f, kernel); e != cudaSuccess)
+                return (int)e;
+            if(f.numRegs != G_LAUNCH_REGS) // the registers would not add up
+                return B200_SGEMM_NO_KERNEL;
+        }
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3(clusters * PAIR * a.split);
-    cfg.blockDim           = dim3(G_THREADS);
+    cfg.blockDim           = dim3(L::THREADS);
     cfg.dynamicSmemBytes   = L::SMEM_BYTES;
     cfg.stream             = stream;
     cudaLaunchAttribute attr[1];
@@ -896,13 +1004,12 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
 }
 
 template<int FMT>
-int launch_tile(int bn, bool pair, const GArgs& a, const Operand& p, const Operand& q, int device, int sms, cudaStream_t stream)
+int launch_tile(int columns, const GArgs& a, const Operand& p, const Operand& q, int device, int sms, cudaStream_t stream)
 {
-    if(pair)
-        return bn == 256 ? launch<FMT, 256, 2>(a, p, q, device, sms, stream) : launch<FMT, 128, 2>(a, p, q, device, sms, stream);
-    if(bn == 64)
-        return launch<FMT, 64, 1>(a, p, q, device, sms, stream);
-    return launch<FMT, 128, 1>(a, p, q, device, sms, stream);
+    if(columns == 256)
+        return a.type == B200_SGEMM_F32 ? launch<FMT, 256, 2, true>(a, p, q, device, sms, stream)
+                                        : launch<FMT, 256, 2>(a, p, q, device, sms, stream);
+    return columns == 64 ? launch<FMT, 64, 1>(a, p, q, device, sms, stream) : launch<FMT, 128, 1>(a, p, q, device, sms, stream);
 }
 
 // `a` holds what both entries agree on; `columns` is the expected number of rows of Q in a group
@@ -911,27 +1018,14 @@ int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_
     int device = 0, sms = 0, status = device_sms(&device, &sms);
     if(status != B200_SGEMM_OK)
         return status;
-    a.K       = (int)K;
-    a.kblocks = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
-    a.chunk   = a.type == B200_SGEMM_F32 ? CHUNK_F32 : a.kblocks;
-    a.bands_p = (a.np + MX4_BAND - 1) / MX4_BAND;
-    int  bn   = columns <= 64 ? 64 : 128;
-    bool pair = false;
-    // one product of few tiles: split K, and where K is too short for that halve the tiles as long as they fit on the SMs at once
-    // (1000 x 1030 x 515: 72 tiles of 128 columns 6.8 us, 144 of 64 see below)
-    auto tiles = [&](int n) { return ((unsigned long long)a.np + G_LANES - 1) / G_LANES * ((columns + n - 1) / n); };
-    if(a.groups == 0 && tiles(64) <= (unsigned long long)sms && split_of(tiles(128), a.kblocks, sms) == 1)
-        bn = 64;
-    // pairs where they fill the SMs
-    const size_t groups = a.groups ? a.groups : 1;
-    const size_t pairs  = ((size_t)a.np + 255) / 256 * ((columns + 255) / 256) * groups;
-    if(columns > 128 && pairs >= (size_t)sms / 2)
-    {
-        pair = true;
-        bn   = a.type == B200_SGEMM_F32 ? 128 : 256;
-    }
-    return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(bn, pair, a, p, q, device, sms, stream)
-                                      : launch_tile<B200_SGEMM_MXFP4>(bn, pair, a, p, q, device, sms, stream);
+    a.K           = (int)K;
+    a.kblocks     = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
+    a.bands_p     = (a.np + MX4_BAND - 1) / MX4_BAND;
+    const Cut cut = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, a.groups == 0, sms);
+    a.split       = cut.split;
+    a.chunk       = a.type != B200_SGEMM_F32 ? a.kblocks : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
+    return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(cut.columns, a, p, q, device, sms, stream)
+                                      : launch_tile<B200_SGEMM_MXFP4>(cut.columns, a, p, q, device, sms, stream);
 }
 } // namespace
 
