@@ -332,7 +332,7 @@ int b200_sgemm_mx4_dequantize(int format, int type, const void* codes, const voi
                               const float* global_scale, void* X, size_t ldx, void* cuda_stream);
 
 /* C[m, n] = alpha * global_a * global_b * sum_k A[m, k] B[n, k] from two quantised matrices of the same format, A of M and
- * B of N rows of K.  C is of `type_c`, row-major (ldc >= N) or col-major (ldc >= M; 0 = packed), overwritten.  Sums are kept
+ * B of N rows of K.  C is of `type_c`, row-major (ldc >= N) or col-major (ldc >= M; 0 = packed), overwritten, and overlaps no operand.  Sums are kept
  * in FP32 and rounded to type_c once.  global_a / global_b: one device float each or NULL (1); NULL for MXFP4.  A few rows on
  * one side (the tokens of a decode step) are a case of its own: the long matrix streams through at the memory's rate. */
 int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
@@ -344,8 +344,9 @@ int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, const void* a_
  * A: rows x K quantised once; B: `groups` matrices of N x K, codes one after the other and scales one after the other (each
  * as its own b200_sgemm_mx4_code_bytes / _scale_bytes); global_b: one float per group.  C: rows x N, row-major, ldc >= N;
  * rows in no group are left as they were.  offsets and counts live on the device, so nothing waits for the host; offsets are
- * multiples of 128 (b200_sgemm_route_sort with align = 128 makes them so), groups without rows cost nothing.  A group whose
- * offset or count does not fit is left out and reported by b200_sgemm_mx4_device_status.  used_rows (0: not known): about how
+ * multiples of 128 (b200_sgemm_route_sort with align = 128 makes them so), groups without rows cost nothing and groups do not
+ * overlap.  A group whose offset or count does not fit is left out and reported by b200_sgemm_mx4_device_status; groups that hold
+ * more rows than the matrix are all left out.  used_rows (0: not known): about how
  * many rows the groups hold in all; it only chooses the tile. */
 int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
                            const void* b_scales, size_t rows, size_t N, size_t K, size_t ldc, size_t groups, const int* offsets,

@@ -113,6 +113,7 @@ struct GArgs
     int            K, kblocks, chunk;
     int            tiles_p, bands_p; // lane tiles; bands of scales of one group's P
     int            groups;  // 0: one product
+    int            most_q;  // column tiles that groups can have in all
     int            split;   // CTAs of a cluster that share a tile
     int            type;
 };
@@ -488,7 +489,8 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
         __syncthreads();
         if(warp == G_TMA_WARP)
         {
-            int sum = 0;
+            int  sum = 0;
+            bool fits = true; // groups that do not overlap have no more tiles than that
             for(int e0 = 0; e0 < a.groups; e0 += 32)
             {
                 const int e = e0 + lane, n = e < a.groups ? first_tile[e] : 0;
@@ -503,9 +505,14 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
                 if(e < a.groups)
                     first_tile[e] = sum + up - n;
                 sum += __shfl_sync(0xFFFFFFFFu, up, 31);
+                fits = fits && sum <= a.most_q;
             }
             if(lane == 0)
-                first_tile[a.groups] = sum;
+            {
+                first_tile[a.groups] = fits ? sum : 0;
+                if(!fits && blockIdx.x == 0)
+                    atomicOr(&g_mx4_status, G_ERR_GROUP);
+            }
         }
     }
     tc_fence_before();
@@ -965,10 +972,11 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
     a.k_tiles  = (int)k_tiles;
     a.tiles_p = (a.np + L::TILE_P - 1) / L::TILE_P;
     // no more than these hold rows: groups start on multiples of 128, for wider tiles each can add one
-    unsigned long long tiles_q = ((unsigned long long)a.nq + BN - 1) / BN + (BN > MX4_BAND ? a.groups : 0);
-    const unsigned long long tiles = tiles_q * a.tiles_p;
+    const unsigned long long tiles_q = ((unsigned long long)a.nq + BN - 1) / BN + (BN > MX4_BAND ? a.groups : 0);
+    const unsigned long long tiles   = tiles_q * a.tiles_p;
     if(tiles > 0x7fffffffull)
         return B200_SGEMM_UNSUPPORTED_SIZE;
+    a.most_q = (int)tiles_q;
     // one tile per cluster where K is split, otherwise as many CTAs as there are tiles or SMs
     const unsigned clusters = (unsigned)(a.split > 1 || tiles < (unsigned long long)(sms / PAIR) ? tiles : sms / PAIR);
     static std::atomic<unsigned long long> ready{0}; // devices on which the kernel may have its shared memory

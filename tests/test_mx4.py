@@ -265,7 +265,7 @@ def check(got, want, bound):
 
 
 SHAPES = [(1, 1, 1), (1, 128, 64), (3, 5, 7), (128, 128, 256), (17, 130, 100), (33, 257, 515), (65, 64, 320), (129, 300, 1000),
-          (200, 520, 2048), (1, 700, 4096), (20, 256, 8192), (300, 2, 777), (4, 129, 2048), (3, 1000, 5000), (2100, 1, 96), (2, 4, 33), (4, 4, 640), (5, 300, 4096), (1000, 16, 200), (512, 640, 130)]
+          (200, 520, 2048), (1, 700, 4096), (20, 256, 8192), (300, 2, 777), (4, 129, 2048), (3, 1000, 5000), (2100, 1, 96), (2, 4, 33), (4, 4, 640), (5, 300, 4096), (40, 50, 1), (200, 100, 31), (1, 3, 9000), (1000, 16, 200), (512, 640, 130)]
 
 
 @gpu
@@ -440,6 +440,11 @@ def test_grouped_leaves_out_groups_that_do_not_fit(sgemm):
         check(c[at], want, ref.product_bound(a[2][at], b[2][e], want, "f32"))
         c[at] = 3
     assert (c == 3).all()
+    # groups on top of each other: more tiles than the rows make
+    c = torch.full((rows, N), 3.0, device="cuda")
+    sgemm.gemm_mx4_grouped(ref.NVFP4, pkg.m_type.f32, c, a[0], a[1], b[0], b[1], rows, N, K, 6, dev(np.zeros(6, np.int32)),
+                           dev(np.full(6, rows, np.int32)))
+    assert sgemm.mx4_device_status() == 2 and (c == 3).all()
 
 
 # ---- as a program uses them ------------------------------------------------------------------------------------------
