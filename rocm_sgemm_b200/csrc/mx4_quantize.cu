@@ -93,18 +93,19 @@ __device__ __forceinline__ Scale scale_mxfp4(unsigned amax_bits)
 // what a code 0..7 stands for
 __device__ __forceinline__ float e2m1_value(unsigned code) { return __uint_as_float(code << 22) * 0x1p126f; }
 
-// the codes nearest to y[0..15], eight bytes
-__device__ __forceinline__ uint2 codes16(const float2 (&y)[Q_LANE_K / 2])
+// the codes nearest to y[0..7], four bytes, without moving bytes by hand
+__device__ __forceinline__ unsigned codes8(const float2* y)
 {
-    uint2 out = make_uint2(0u, 0u);
-#pragma unroll
-    for(int i = 0; i < 4; ++i)
-    {
-        out.x |= (unsigned)__nv_cvt_float2_to_fp4x2(y[i], __NV_E2M1, cudaRoundNearest) << (8 * i);
-        out.y |= (unsigned)__nv_cvt_float2_to_fp4x2(y[4 + i], __NV_E2M1, cudaRoundNearest) << (8 * i);
-    }
-    return out;
+    unsigned r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r)
+        : "f"(y[0].x), "f"(y[0].y), "f"(y[1].x), "f"(y[1].y), "f"(y[2].x), "f"(y[2].y), "f"(y[3].x), "f"(y[3].y));
+    return r;
 }
+__device__ __forceinline__ uint2 codes16(const float2 (&y)[Q_LANE_K / 2]) { return make_uint2(codes8(y), codes8(y + 4)); }
 // y = x * f, two values an instruction
 __device__ __forceinline__ void scaled16(float2 (&y)[Q_LANE_K / 2], const float (&x)[Q_LANE_K], float f)
 {
