@@ -5,11 +5,11 @@
 
 namespace sgemm_b200
 {
-// whether mx4_few takes the product: one row, or two against a matrix of which they cost less than the tensor core's set-up
-// (measured: two rows x 4096 x 4096 6.1 us against 7.4, x 16384 x 4096 17 us against 11; one row 4.6 against 7.3, 11.2 against 10.9)
+// whether mx4_few takes the product: one or two rows against a matrix of which they cost less than the tensor core's set-up
+// (measured: one row x 4096 x 4096 4.0 us against 7.3, x 16384 x 4096 11.1 us against 10.9; two rows 5.2 against 7.4, 17 against 11)
 inline bool mx4_is_few(size_t few, size_t rows, size_t K)
 {
-    return few == 1 ? rows * K <= (size_t(1) << 26) : few == 2 && rows * K <= (size_t(1) << 24);
+    return few == 1 ? rows * K <= (size_t(1) << 25) : few == 2 && rows * K <= (size_t(1) << 24);
 }
 
 struct FewArgs

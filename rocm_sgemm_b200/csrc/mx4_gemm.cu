@@ -88,7 +88,7 @@ struct GLayout
     static constexpr int    ACCS        = BN > 128 ? 1 : 2; // accumulators
     static constexpr int    BARRIERS    = 2 * STAGES + 6;
     static constexpr size_t SMEM_BYTES  = size_t(STAGES) * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers, misc*/;
-    static_assert(8 * BARRIERS + 16 <= 256, "barrier area");
+    static_assert(8 * BARRIERS + 16 <= 256 && BARRIERS <= 32, "barrier area, a lane each");
     static_assert(ACCS * BN <= G_SCALE_COL, "tensor memory");
     static_assert(BN % 64 == 0 && SLOT_COLS % 4 == 0 && TILES % 2 == 0, "scales start on an even column");
     static_assert(SMEM_BYTES + (G_MAX_GROUPS + 1) * 4 <= 227 * 1024, "shared memory");
@@ -114,7 +114,7 @@ struct GArgs
     int            tiles_p, bands_p; // lane tiles; bands of scales of one group's P
     int            groups;  // 0: one product
     int            most_q;  // column tiles that groups can have in all
-    int            split;   // CTAs of a cluster that share a tile
+    int            split_bits; // 2^split_bits CTAs of a cluster share a tile
     int            type;
 };
 
@@ -301,10 +301,29 @@ __device__ __forceinline__ void store_columns(const GArgs& a, const float (&acc)
     }
     else
     {
+        // eight columns at a time, without a test each where all are there (a test, a 64-bit product and a branch for each of 32
+        // columns took 0.8 us)
+        constexpr int STEP = 8;
+        const int     n    = q_end - q0;
 #pragma unroll
-        for(int j = 0; j < COLS; ++j)
-            if(q0 + j < q_end)
-                c[(long long)j * a.sq] = from_float<T>(acc[j] * factor);
+        for(int j0 = 0; j0 < COLS; j0 += STEP)
+        {
+            if(j0 >= n)
+                break;
+            if(j0 + STEP <= n)
+            {
+#pragma unroll
+                for(int j = 0; j < STEP; ++j, c += a.sq)
+                    *c = from_float<T>(acc[j0 + j] * factor);
+            }
+            else
+            {
+#pragma unroll
+                for(int j = 0; j < STEP; ++j, c += a.sq)
+                    if(j0 + j < n)
+                        *c = from_float<T>(acc[j0 + j] * factor);
+            }
+        }
     }
 }
 template<int COLS>
@@ -374,10 +393,27 @@ __device__ __forceinline__ void store_packed(const GArgs& a, const uint32_t (&v)
     }
     else
     {
+        constexpr int STEP = 16;
+        const int     n    = q_end - q0;
 #pragma unroll
-        for(int j = 0; j < COLS; ++j)
-            if(q0 + j < q_end)
-                c[(long long)j * a.sq] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+        for(int j0 = 0; j0 < COLS; j0 += STEP)
+        {
+            if(j0 >= n)
+                break;
+            if(j0 + STEP <= n)
+            {
+#pragma unroll
+                for(int j = 0; j < STEP; ++j, c += a.sq)
+                    *c = (uint16_t)(v[(j0 + j) / 2] >> (16 * (j & 1)));
+            }
+            else
+            {
+#pragma unroll
+                for(int j = 0; j < STEP; ++j, c += a.sq)
+                    if(j0 + j < n)
+                        *c = (uint16_t)(v[(j0 + j) / 2] >> (16 * (j & 1)));
+            }
+        }
     }
 }
 
@@ -403,12 +439,12 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
     volatile int*  abort_flag = reinterpret_cast<volatile int*>(misc + 8);
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int split = a.split, shared_by = PAIR * split; // CTAs of the cluster
-    const int rank  = shared_by > 1 ? (int)(blockIdx.x % shared_by) : 0;
+    const int split = 1 << a.split_bits, shared_by = PAIR * split; // CTAs of the cluster, a power of two
+    const int rank  = (int)(blockIdx.x & (shared_by - 1));
     const int lane0 = PAIR > 1 ? rank * G_LANES : 0; // this CTA's first lane in the tile
-    const int first = blockIdx.x / shared_by, stride = gridDim.x / shared_by;
+    const int first = blockIdx.x >> (a.split_bits + PAIR - 1), stride = gridDim.x >> (a.split_bits + PAIR - 1);
     const int part  = PAIR > 1 ? 0 : rank; // this CTA's range of K
-    const int kb0 = (int)((long long)a.kblocks * part / split), kb1 = (int)((long long)a.kblocks * (part + 1) / split);
+    const int kb0 = (a.kblocks * part) >> a.split_bits, kb1 = (a.kblocks * (part + 1)) >> a.split_bits; // kblocks < 2^23
     // one stage of a tile: codes and scales of K block kb
     auto fill = [&](const Tile& t, int kb, int s) {
         const uint32_t st  = base + s * L::STAGE_BYTES;
@@ -440,21 +476,12 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
     {
         if(lane < (int)(sizeof(maps) / sizeof(CUtensorMap))) // the descriptors at once: each costs a trip to memory
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.p + lane)) : "memory");
-        if(lane == 0)
+        if(lane < L::BARRIERS) // one each: full, empty, acc_full, acc_empty, drained, parts
         {
-            for(int s = 0; s < STAGES; ++s)
-            {
-                mbar_init(full(s), 1);
-                mbar_init(empty(s), 1);
-            }
-            for(int b = 0; b < 2; ++b)
-            {
-                mbar_init(acc_full(b), 1);
-                mbar_init(acc_empty(b), PAIR * G_EPILOGUE / 32);
-            }
-            mbar_init(drained, 1);
-            mbar_init(parts, 1);
-            *abort_flag = 0;
+            const bool of_epilogue = lane >= 2 * STAGES + 2 && lane < 2 * STAGES + 4;
+            mbar_init(bar_base + 8u * lane, of_epilogue ? PAIR * G_EPILOGUE / 32 : 1);
+            if(lane == 0)
+                *abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -978,7 +1005,8 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
         return B200_SGEMM_UNSUPPORTED_SIZE;
     a.most_q = (int)tiles_q;
     // one tile per cluster where K is split, otherwise as many CTAs as there are tiles or SMs
-    const unsigned clusters = (unsigned)(a.split > 1 || tiles < (unsigned long long)(sms / PAIR) ? tiles : sms / PAIR);
+    const int      split    = 1 << a.split_bits;
+    const unsigned clusters = (unsigned)(split > 1 || tiles < (unsigned long long)(sms / PAIR) ? tiles : sms / PAIR);
     static std::atomic<unsigned long long> ready{0}; // devices on which the kernel may have its shared memory
     const unsigned long long               bit = 1ull << (device % MAX_DEVICES);
     if(device >= MAX_DEVICES || !(ready.load(std::memory_order_relaxed) & bit))
@@ -997,17 +1025,17 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3(clusters * PAIR * a.split);
+    cfg.gridDim            = dim3(clusters * PAIR * split);
     cfg.blockDim           = dim3(L::THREADS);
     cfg.dynamicSmemBytes   = L::SMEM_BYTES;
     cfg.stream             = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id               = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)(PAIR * a.split);
+    attr[0].val.clusterDim.x = (unsigned)(PAIR * split);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs                = attr;
-    cfg.numAttrs             = PAIR * a.split > 1 ? 1 : 0;
+    cfg.numAttrs             = PAIR * split > 1 ? 1 : 0;
     return (int)cudaLaunchKernelEx(&cfg, kernel, a, maps);
 }
 
@@ -1030,7 +1058,8 @@ int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_
     a.kblocks     = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
     a.bands_p     = (a.np + MX4_BAND - 1) / MX4_BAND;
     const Cut cut = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, a.groups == 0, sms);
-    a.split       = cut.split;
+    while((1 << a.split_bits) < cut.split)
+        ++a.split_bits;
     a.chunk       = a.type != B200_SGEMM_F32 ? a.kblocks : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
     return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(cut.columns, a, p, q, device, sms, stream)
                                       : launch_tile<B200_SGEMM_MXFP4>(cut.columns, a, p, q, device, sms, stream);
