@@ -348,6 +348,17 @@ struct Maps<1>
     CUtensorMap p, q;
 };
 
+// Columns that the instructions of a tile compute: the last tile of a group seldom needs all (32 experts of about 1024 rows x 4096
+// x 2048: 129.7 us, 131.7 with all).  The CTAs of a pair hold the rows of the first and the second half of them.
+template<int BN, int PAIR>
+__device__ __forceinline__ int columns_of(const Tile& t)
+{
+    const int left = t.q_end - t.q0;
+    if(PAIR > 1)
+        return min(BN, (left + 63) / 64 * 64);
+    return BN == 64 && left <= 32 ? 32 : BN;
+}
+
 // the first n of N results, `stride` elements apart
 template<class T, int N>
 __device__ __forceinline__ void store_strided(T* c, const float (&v)[N], float factor, long long stride, int n)
@@ -357,17 +368,7 @@ __device__ __forceinline__ void store_strided(T* c, const float (&v)[N], float f
         if(j < n)
             c[j * stride] = from_float<T>(v[j] * factor);
 }
-// two results of 16 bits as they are stored, the first in the lower half
-__device__ __forceinline__ uint32_t pack16(int type, float x, float y)
-{
-    if(type == B200_SGEMM_F16)
-    {
-        const __half2 h = __floats2half2_rn(x, y);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
+// results of 16 bits, two in a word, the first in the lower half
 template<int COLS>
 __device__ __forceinline__ void store_packed(const GArgs& a, const uint32_t (&v)[COLS / 2], int p, int q0, int q_end)
 {
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
     auto fill = [&](const Tile& t, int kb, int s) {
         const uint32_t st  = base + s * L::STAGE_BYTES;
         const uint32_t bar = PAIR > 1 ? cluster_addr(full(s), 0) : full(s);
-        const bool     whole = L::Q_BOX == L::Q_ROWS || t.q0 + L::Q_BOX < t.q_end; // or the first box alone
+        const bool     whole = L::Q_BOX == L::Q_ROWS || columns_of<BN, PAIR>(t) > L::Q_BOX; // or the first box alone
         // a pair's copies bring whole stages (zero beyond the matrix), a single CTA's the tiles that there are
         const int      tiles = PAIR > 1 ? L::TILES : min(L::TILES, a.k_tiles - kb * L::TILES);
         const int      band_p = t.group * a.bands_p + (t.p0 + lane0) / MX4_BAND, band_q = t.q0 / MX4_BAND;
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
         if(rank == 0 || PAIR == 1)
             mbar_arrive_expect_tx(full(s), PAIR * (L::P_BYTES + (whole ? L::Q_BYTES : L::BOX_BYTES) + bytes * (1 + L::Q_BANDS)));
         load_codes<PAIR>(st, &maps.p, kb * G_ROW_BYTES, t.group * a.np + t.p0 + lane0, bar);
-        load_codes<PAIR>(st + L::P_BYTES, &maps.q, kb * G_ROW_BYTES, t.q0 + (PAIR > 1 ? rank * L::Q_ROWS : 0), bar);
+        load_codes<PAIR>(st + L::P_BYTES, &maps.q, kb * G_ROW_BYTES, t.q0 + (PAIR > 1 ? rank * (columns_of<BN, PAIR>(t) / 2) : 0), bar);
         if(L::Q_BOX < L::Q_ROWS && whole)
             load_codes<PAIR>(st + L::P_BYTES + L::BOX_BYTES, &maps.q, kb * G_ROW_BYTES, t.q0 + L::Q_BOX, bar);
         if constexpr(PAIR > 1)
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
             const Tile     t     = tile_at<BN, L::TILE_P>(a, first_tile, tile);
             // Q's rows start at column q_col of the band's scales: 0, or 2 for the second tile of 64 (an odd column is a fault)
             const uint32_t q_col = t.q0 % MX4_BAND / 32;
-            const uint32_t idesc = mx4_idesc<FMT, PAIR>(L::Q_BOX < L::Q_ROWS && t.q0 + L::Q_BOX >= t.q_end ? L::Q_BOX : BN);
+            const uint32_t idesc = mx4_idesc<FMT, PAIR>(columns_of<BN, PAIR>(t));
             int            in_chunk = 0;
             for(int kb = kb0; kb < kb1; ++kb)
             {
@@ -683,20 +684,31 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_
                 if(!warp_wait(acc_full(0), acc_ph, abort_flag)) { fail(3); ok = false; break; }
                 tc_fence_after();
                 const uint32_t from = tmem_base + half * COLS + (uint32_t(quarter * 32) << 16);
+                auto empty_into = [&](auto pack) { // packed while the next 32 columns are on their way
+                    uint32_t v[2][32];
+                    tmem_ld32(from, v[0]);
 #pragma unroll
-                for(int c = 0; c < COLS; c += 32)
-                {
-                    uint32_t v[32];
-                    tmem_ld32(from + c, v);
-                    tmem_ld_wait();
+                    for(int c = 0; c < COLS; c += 32)
+                    {
+                        tmem_ld_wait();
+                        if(c + 32 < COLS)
+                            tmem_ld32(from + c + 32, v[(c / 32 + 1) % 2]);
+                        else
+                        {
+                            tc_fence_before();
+                            __syncwarp();
+                            if(lane == 0)
+                                mbar_arrive_cluster(cluster_addr(acc_empty(0), 0));
+                        }
 #pragma unroll
-                    for(int j = 0; j < 32; j += 2)
-                        out[(c + j) / 2] = pack16(a.type, __uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor);
-                }
-                tc_fence_before();
-                __syncwarp();
-                if(lane == 0)
-                    mbar_arrive_cluster(cluster_addr(acc_empty(0), 0));
+                        for(int j = 0; j < 32; j += 2)
+                            out[(c + j) / 2] = pack(__uint_as_float(v[c / 32 % 2][j]) * factor, __uint_as_float(v[c / 32 % 2][j + 1]) * factor);
+                    }
+                };
+                if(a.type == B200_SGEMM_F16)
+                    empty_into([](float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); });
+                else
+                    empty_into([](float x, float y) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); });
                 acc_ph ^= 1;
                 store_packed<COLS>(a, out, t.p0 + lane0 + quarter * 32 + lane, t.q0 + half * COLS, t.q_end);
                 continue;
@@ -943,23 +955,25 @@ struct Cut
 {
     int columns, split;
 };
-// The cut with the least estimated time, from what a few dozen shapes between 100 x 1000 x 300 and 2560^3 measured (us, BF16
-// result): a K block takes 0.33 / 0.37 / 0.37 in tiles of 64 / 128 / 256 columns, for the SMs go through it at about the same pace
-// whatever its width; storing a tile 1.3 / 2.4 / 2.5 where the next tile's blocks do not hide it, and 0.5 / 1 / 2 more at the end;
-// adding the parts of a split tile 1.4 / 2.4 for 64 / 128 columns.  Examples, us for (columns, split): 2048^3 (128, 1) 12.6,
-// (256, 1) 9.8; 128 x 8192 x 8192 (64, 1) 15.3, (128, 2) 14.5, (256, 1) 16.3; 512 x 512 x 8192 (64, 1) 14.2, (64, 4) 10.1;
-// 512^3 (64, 1) 5.8, (64, 2) 7.2, (128, 1) 6.7.
+// The cut with the least estimated time, from what two dozen shapes between 100 x 1000 x 300 and 2560^3 measured (us): a K block
+// takes 0.33 / 0.37 / 0.37 in tiles of 64 / 128 / 256 columns, for the SMs go through it at about the same pace whatever
+// its width; storing a tile 1.1 / 1.75 / 2.3 where the next tile's blocks do not hide it, and 0.4 / 0.9 / 2 more at the end; FP32
+// results in 256 columns, which are added in registers, 0.4 a block, 3.7 and 3.5; adding the parts of a split tile 2.2 / 3.3.
+// Examples, us for (columns, split), BF16: 2048^3 (128, 1) 11.5, (256, 1) 9.1; 64 x 8192 x 8192 (64, 1) 13.9, (64, 2) 12.1,
+// (128, 2) 12.9; 512 x 512 x 8192 (64, 1) 13.5, (64, 4) 9.7; 512^3 (64, 1) 4.7, (64, 2) 7.0, (128, 1) 5.4.
 // lane_rows, column_rows: extents of one group; clusters of 8 and 4 CTAs do not fill every part of the chip, so they are held
 // below three quarters and seven eighths of the SMs.
-Cut cut_of(size_t lane_rows, size_t column_rows, size_t groups, int kblocks, bool may_split, int sms)
+Cut cut_of(size_t lane_rows, size_t column_rows, size_t groups, int kblocks, bool f32, bool may_split, int sms)
 {
     Cut   best = {64, 1};
     float least = 1e30f;
     for(int i = 0; i < 3; ++i)
     {
         const int    columns = 64 << i, lanes = i == 2 ? 256 : 128, slots = i == 2 ? sms / 2 : sms;
-        const float  block = i == 0 ? 0.33f : 0.37f, store = i == 0 ? 1.3f : (i == 1 ? 2.4f : 2.5f);
-        const float  end = i == 0 ? 0.5f : (i == 1 ? 1.f : 2.f), join = i == 0 ? 1.4f : 2.4f;
+        const bool   sums  = f32 && i == 2;
+        const float  block = i == 0 ? 0.33f : (sums ? 0.4f : 0.37f), join = i == 0 ? 2.2f : 3.3f;
+        const float  store = i == 0 ? 1.1f : (i == 1 ? 1.75f : (sums ? 3.7f : 2.3f));
+        const float  end   = i == 0 ? 0.4f : (i == 1 ? 0.9f : (sums ? 3.5f : 2.f));
         const size_t tiles = (lane_rows + lanes - 1) / lanes * ((column_rows + columns - 1) / columns) * groups;
         for(int split = 1; split <= (may_split && i < 2 ? MAX_SPLIT : 1); split *= 2)
         {
@@ -1057,7 +1071,7 @@ int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_
     a.K           = (int)K;
     a.kblocks     = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
     a.bands_p     = (a.np + MX4_BAND - 1) / MX4_BAND;
-    const Cut cut = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, a.groups == 0, sms);
+    const Cut cut = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, a.type == B200_SGEMM_F32, a.groups == 0, sms);
     while((1 << a.split_bits) < cut.split)
         ++a.split_bits;
     a.chunk       = a.type != B200_SGEMM_F32 ? a.kblocks : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
