@@ -59,8 +59,8 @@ constexpr int CHUNK_F32_WIDE = 8; // the same for 256 columns, whose one accumul
 constexpr int G_LAUNCH_REGS = 168, G_SUM_REGS = 224, G_ISSUE_REGS = 56;
 static_assert(G_EPILOGUE * G_SUM_REGS + 128 * G_ISSUE_REGS == (G_EPILOGUE + 128) * G_LAUNCH_REGS, "register budgets");
 
-constexpr int G_ERR_WAIT  = 1; // status bits: a wait gave up (bits 8.. say which);
-constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the matrix, the group was left out
+constexpr int G_ERR_WAIT  = 1; // status bits: a wait gave up (bits 8.. say which)
+constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the matrix, and the group was left out
 
 __device__ int g_mx4_status;
 
@@ -99,10 +99,10 @@ struct GLayout
 struct GArgs
 {
     void*          c;
-    long long      sp, sq; // element strides of C along lanes and columns; one of them is 1
+    long long      sp, sq;   // element strides of C along lanes and columns; one of them is 1
     const uint8_t* scales_p; // for a single CTA, which takes the tiles by plain bulk copies (two descriptors less to build: 0.6 us)
     const uint8_t* scales_q;
-    int            k_tiles;  // scale tiles along k
+    int            k_tiles; // scale tiles along k
     const int*     offsets; // grouped: first row (of Q and C) of each group, and rows
     const int*     counts;
     const float*   global_p;
@@ -419,7 +419,8 @@ __device__ __forceinline__ void store_packed(const GArgs& a, const uint32_t (&v)
 }
 
 template<int FMT, int BN, int PAIR, bool SUMS>
-__global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1) mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ Maps<PAIR> maps)
+__global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1)
+    mx4_gemm_kernel(const __grid_constant__ GArgs a, const __grid_constant__ Maps<PAIR> maps)
 {
     using L = GLayout<FMT, BN, PAIR, SUMS>;
     constexpr int STAGES = L::STAGES;
@@ -1015,7 +1016,7 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
     // no more than these hold rows: groups start on multiples of 128, for wider tiles each can add one
     const unsigned long long tiles_q = ((unsigned long long)a.nq + BN - 1) / BN + (BN > MX4_BAND ? a.groups : 0);
     const unsigned long long tiles   = tiles_q * a.tiles_p;
-    if(tiles > 0x7fffffffull)
+    if(tiles > 0x3fffffffull) // the CTAs step beyond the last one
         return B200_SGEMM_UNSUPPORTED_SIZE;
     a.most_q = (int)tiles_q;
     // one tile per cluster where K is split, otherwise as many CTAs as there are tiles or SMs
