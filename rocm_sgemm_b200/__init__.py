@@ -182,8 +182,10 @@ def _check(status: int) -> None:
 def _ptr(x) -> int:
     if x is None:
         return 0
-    data_ptr = getattr(x, "data_ptr", None)
-    return data_ptr() if data_ptr is not None else int(x)
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return int(x)
 
 
 _raw_stream = None  # () -> the current torch stream's handle, once torch has a CUDA device

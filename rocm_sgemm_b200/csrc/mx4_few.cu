@@ -4,7 +4,7 @@
 //
 // Bound by HBM: the long matrix is read once, 4.5 bits a value, and there are only 2 x `few` operations for each.  The tensor
 // core's way (mx4_gemm.cu) brings little here: it copies scale tiles into tensor memory at 50 cycles each, as many for one
-// token as for 128, and its set-up and split of K cost as much as the work: 7.3 us for 1 x 4096 x 4096.
+// token as for 128, and its set-up and split of K cost as much as the work: 7.0 us for 1 x 4096 x 4096.
 //
 // Products of two e2m1 values are multiples of 1/4 up to 36, so the sum of eight is exact in FP16 (1152 quarters): a block of 16
 // is eight fused multiply-adds on pairs, whose two halves are added in FP32.  That sum has at most 12 bits, with both scales at
@@ -16,7 +16,7 @@
 // the other's are used.  Long matrices of few rows: the warps of a CTA share rows and split K; sums are then added in the
 // warps' order.  What is left is the arithmetic on the way (some 70 instructions for 32 values of a lane, a quarter of them
 // conversions) and the registers it takes, which leave two CTAs an SM: one row x 4096 x 4096 takes 4.0 us, where the tensor core
-// takes 7.3; 1 x 16384 x 4096 11.1 us, where it takes 10.9.  One group a warp and three CTAs: 5.1 and 14.4 us.
+// takes 7.0; 1 x 16384 x 4096 11.1 us, where it takes 10.1.  One group a warp and three CTAs: 5.1 and 14.4 us.
 #include "mx4_few.hpp"
 
 #include "mx4_common.cuh"
@@ -29,7 +29,6 @@ constexpr int F_THREADS = 256;
 constexpr int F_WARPS   = F_THREADS / 32;
 constexpr int F_LANE_K  = 32;
 constexpr int F_GROUPS  = 2; // of four rows, that a warp takes
-
 
 struct Args
 {

@@ -6,7 +6,8 @@
 namespace sgemm_b200
 {
 // whether mx4_few takes the product: one or two rows against a matrix of which they cost less than the tensor core's set-up
-// (measured: one row x 4096 x 4096 4.0 us against 7.3, x 16384 x 4096 11.1 us against 10.9; two rows 5.2 against 7.4, 17 against 11)
+// (measured: one row x 4096 x 4096 4.0 us against 7.0, x 16384 x 4096 11.1 us against 10.1; two rows 5.2 against 7.0, 17 against
+// 10.2)
 inline bool mx4_is_few(size_t few, size_t rows, size_t K)
 {
     return few == 1 ? rows * K <= (size_t(1) << 25) : few == 2 && rows * K <= (size_t(1) << 24);

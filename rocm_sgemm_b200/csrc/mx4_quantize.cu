@@ -11,9 +11,10 @@
 //   * the scale: the quotient in FP32 is off by a few units, so its rounding is off by one step at most; the sign of
 //     amax - 6 m g for the midpoints m on both sides of it, which one fused multiply-add gives exactly (6 m has seven
 //     bits), says whether to move.
-//   * the codes, g with at most 17 significant bits (1.0, powers of two): s g is exact in 21 bits, so every midpoint
-//     t s g is an FP32 number; the correctly rounded quotient (one product and two fused multiply-adds) is then on the
-//     same side of t as x / (s g), or on t when that is.
+//   * the codes, g with at most 12 significant bits (1.0, powers of two): s g is exact in 16 bits and every midpoint t s g an
+//     FP32 number, which the next FP32 number x is so far from that the quotient in FP32 (one product and two fused
+//     multiply-adds, off by 2^-45 before its rounding) is t only if x / (s g) is: the closest case, t = 1/4 and s g just below a
+//     power of two, leaves 2^-40.
 //   * any other g: products with the reciprocal, made a little too small and a little too large (2^-21, five roundings of
 //     2^-24 lie in between), bracket the quotient.  Where their codes differ the value is read again and the sign of
 //     |x| - (t s) g decides, exact as above.  That is rare for random g, but g = amax / 2688 of BF16 data makes every
@@ -41,7 +42,7 @@ constexpr unsigned INF_BITS  = 0x7F800000u;
 struct Global
 {
     float g, r6;   // 1 / (6 g)
-    bool  ok, few; // ok: finite and in 2^+-90, where none of the products below can leave FP32's range; few: <= 17 bits
+    bool  ok, few; // ok: finite and in 2^+-90, where none of the products below can leave FP32's range; few: <= 12 bits
 };
 __device__ __forceinline__ Global load_global(const float* p)
 {
@@ -49,7 +50,7 @@ __device__ __forceinline__ Global load_global(const float* p)
     G.g   = p ? *p : 1.f;
     G.r6  = __frcp_rn(6.f * G.g);
     G.ok  = G.g >= 0x1p-90f && G.g <= 0x1p90f;
-    G.few = (__float_as_uint(G.g) & 0x7Fu) == 0;
+    G.few = (__float_as_uint(G.g) & 0xFFFu) == 0;
     return G;
 }
 

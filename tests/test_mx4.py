@@ -125,15 +125,13 @@ def test_grouped_refuses(sgemm):
 # ---- quantisation ----------------------------------------------------------------------------------------------------
 
 @gpu
-@pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
+@pytest.mark.parametrize("fmt,g", [(ref.MXFP4, None), (ref.NVFP4, None), (ref.NVFP4, 0.125), (ref.NVFP4, 0.0123)],
+                         ids=lambda v: ("nvfp4", "mxfp4")[v] if isinstance(v, int) else str(v))
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("layout", [0, 1])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 16), (3, 33), (129, 70), (128, 512), (40, 1030), (300, 600)],
                          ids=lambda s: "x".join(map(str, s)))
-@pytest.mark.parametrize("g", [None, 0.125, 0.0123], ids=str)
 def test_quantize_is_exact(sgemm, fmt, dtype, layout, shape, g):
-    if fmt == ref.MXFP4 and g is not None:
-        pytest.skip("mxfp4 has no matrix scale")
     rows, K = shape
     x, x64 = source(rows, K, rows * 1000 + K, dtype)
     gt = None if g is None else torch.tensor([g], dtype=torch.float32, device="cuda")
@@ -210,8 +208,10 @@ def test_quantize_bad_matrix_scale_gives_nan(sgemm, g):
 def test_quantize_borders_of_an_awkward_matrix_scale(sgemm):
     """Values next to the border between two codes, where the quotient in FP32 cannot tell the side."""
     r = np.random.default_rng(3)
-    for trial in range(20):
+    for trial in range(30):
         g = np.float32(r.uniform(0.5, 2.0) * 2.0 ** float(r.integers(-30, 10)))
+        if trial >= 20:  # few bits, and as close below a power of two as 12 or 13 of them come
+            g = np.float32([1.0, 0.75, 2 - 2.0 ** -11, 2 - 2.0 ** -12, 1 + 2.0 ** -11][trial % 5])
         s = ref.E4M3[r.integers(8, 0x7E, (64, 8))]
         mid = r.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], (64, 8, 16))
         x = (mid * s[..., None] * float(g)).astype(np.float32)
@@ -371,18 +371,20 @@ def test_product_exact_sums(sgemm, fmt):
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
-def test_product_of_nan_blocks_is_nan(sgemm, fmt):
-    M, N, K = 40, 200, 300
+@pytest.mark.parametrize("other", [1, 2, 200])
+def test_product_of_nan_blocks_is_nan(sgemm, fmt, other):
+    M, N, K = 40, other, 300
     x = torch.randn(M, K)
     x[7, 290] = float("nan")
-    x[9, 0] = float("inf")
+    x[39, 0] = float("inf")
     a = quantize(sgemm, fmt, x.cuda(), M, K, "f32")
     b = operand(fmt, N, K, 5)
-    c = torch.zeros(M, N, device="cuda")
+    c, t = torch.zeros(M, N, device="cuda"), torch.zeros(N, M, device="cuda")
     sgemm.gemm_mx4(fmt, 0, pkg.m_type.f32, c, a[0], a[1], b[0], b[1], M, N, K)
-    nan = torch.isnan(c)
-    assert nan[7].all() and nan[9].all()
-    assert nan.sum().item() == 2 * N
+    sgemm.gemm_mx4(fmt, 0, pkg.m_type.f32, t, b[0], b[1], a[0], a[1], N, M, K)
+    for nan in (torch.isnan(c), torch.isnan(t.T)):
+        assert nan[7].all() and nan[39].all()
+        assert nan.sum().item() == 2 * N
 
 
 def grouped_case(fmt, counts, N, K, rows=None, seed=0):
@@ -508,4 +510,62 @@ def test_linear_layer_and_its_gradients(sgemm):
     product(x, 0, w, 0, M, N, K)    # y[m, n]: sum over k
     product(dy, 0, w, 1, M, K, N)   # dx[m, k]: sum over n; w's transpose is its columns
     product(dy, 1, x, 1, N, K, M)   # dw[n, k]: sum over m
+    assert sgemm.mx4_device_status() == 0
+
+
+@gpu
+def test_leading_dimensions_beyond_32_bits(sgemm):
+    """Elements whose offset passes 2^31, on every side that takes a leading dimension."""
+    rows, K, ld = 2100, 96, 1 << 20
+    bf16, f32 = pkg.m_type.bf16, pkg.m_type.f32
+    x = torch.randn(rows, K, device="cuda").bfloat16()
+    big = torch.empty(rows, ld, dtype=torch.bfloat16, device="cuda")
+    big[:, :K] = x
+    packed, strided = quantize(sgemm, ref.NVFP4, x, rows, K, "bf16"), quantize(sgemm, ref.NVFP4, big, rows, K, "bf16", ldx=ld)
+    assert all(torch.equal(p, s) for p, s in zip(packed, strided))
+    # columns: K of them 2^20 apart
+    packed_t = quantize(sgemm, ref.MXFP4, x, K, rows, "bf16", 1)
+    strided_t = quantize(sgemm, ref.MXFP4, big, K, rows, "bf16", 1, ldx=ld)
+    assert all(torch.equal(p, s) for p, s in zip(packed_t, strided_t))
+    out = torch.empty(rows, K, dtype=torch.bfloat16, device="cuda")
+    sgemm.mx4_dequantize(ref.NVFP4, bf16, *packed, rows, K, out)
+    big[:, :K] = 0
+    sgemm.mx4_dequantize(ref.NVFP4, bf16, *packed, rows, K, big, ldx=ld)
+    assert torch.equal(big[:, :K], out)
+    w = quantize(sgemm, ref.NVFP4, torch.randn(K, K, device="cuda"), K, K, "f32")
+    for layout_c in (0, 1):
+        c = torch.empty(rows, K, dtype=torch.bfloat16, device="cuda")
+        big[:, :K] = 0
+        a, b, m, n = (packed, w, rows, K) if layout_c == 0 else (w, packed, K, rows)
+        sgemm.gemm_mx4(ref.NVFP4, layout_c, bf16, c, *a, *b, m, n, K)
+        sgemm.gemm_mx4(ref.NVFP4, layout_c, bf16, big, *a, *b, m, n, K, ldc=ld)
+        assert torch.equal(big[:, :K], c)
+    assert sgemm.mx4_device_status() == 0
+
+
+@gpu
+def test_codes_beyond_32_bits(sgemm):
+    """A matrix whose codes take more than 2^32 bytes: its last rows, quantised, read back and multiplied."""
+    rows, K, last = (1 << 17) + 40, 1 << 16, 100
+    bf16 = pkg.m_type.bf16
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device="cuda")
+    tail = torch.randn(last, K, device="cuda").bfloat16()
+    x[-last:] = tail
+    codes, scales = quantize(sgemm, ref.MXFP4, x, rows, K, "bf16")
+    assert codes.numel() > 1 << 32
+    code, byte = ref.quantize(ref.MXFP4, tail.double().cpu().numpy())
+    values = ref.values(ref.MXFP4, code, byte)
+    assert np.array_equal(codes.view(rows, -1)[-last:].cpu().numpy().reshape(-1), ref.pack(ref.MXFP4, code, byte)[0])
+    sgemm.mx4_dequantize(ref.MXFP4, bf16, codes, scales, rows, K, x)
+    assert np.array_equal(x[-last:].double().cpu().numpy(), values)
+    assert not x[:1000].any() and not x[rows // 2:rows // 2 + 1000].any()
+    del x
+    for m in (1, 3):
+        a = operand(ref.MXFP4, m, K, 6)
+        want = a[2] @ values.T
+        bound = ref.product_bound(a[2], values, want, "f32")
+        c = torch.empty(m, rows, device="cuda")
+        sgemm.gemm_mx4(ref.MXFP4, 0, pkg.m_type.f32, c, a[0], a[1], codes, scales, m, rows, K)
+        check(c[:, -last:], want, bound)
+        assert not c[:, :-last].any()
     assert sgemm.mx4_device_status() == 0

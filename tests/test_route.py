@@ -182,6 +182,31 @@ def test_combine_backward(sgemm, dtype, pad, tokens, top_k, width):
 
 
 @gpu
+def test_leading_dimensions_beyond_32_bits(sgemm):
+    tokens, top_k, width, ld = 1100, 2, 64, 1 << 20
+    rows, t = tokens * top_k, pkg.m_type.bf16
+    slot_row = torch.randperm(rows, device="cuda").to(torch.int32)
+    token = torch.arange(rows, device="cuda") // top_k
+    x, w = torch.randn(tokens, width, device="cuda").bfloat16(), torch.rand(tokens, top_k, device="cuda")
+    big = torch.empty(rows, ld, dtype=torch.bfloat16, device="cuda")
+    sgemm.route_dispatch(t, x, tokens, width, slot_row, top_k, big, rows, lds=ld)
+    y = torch.empty(rows, width, dtype=torch.bfloat16, device="cuda")
+    y[slot_row.long()] = x[token]
+    assert torch.equal(big[:, :width], y)
+    outs = [torch.empty(tokens, width, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    sgemm.route_combine(t, big, rows, width, slot_row, tokens, top_k, outs[0], weights=w, ldy=ld)
+    sgemm.route_combine(t, y, rows, width, slot_row, tokens, top_k, outs[1], weights=w)
+    assert torch.equal(*outs)
+    dw, dw_big = torch.empty_like(w), torch.empty_like(w)
+    dy = torch.empty_like(y)
+    sgemm.route_combine_backward(t, x, y, rows, width, slot_row, tokens, top_k, w, dy, dw)
+    sgemm.route_combine_backward(t, x, big, rows, width, slot_row, tokens, top_k, w, None, dw_big, ldy=ld)
+    assert torch.equal(dw, dw_big)
+    sgemm.route_combine_backward(t, x, None, rows, width, slot_row, tokens, top_k, w, big, None, lddy=ld)
+    assert torch.equal(big[:, :width], dy)
+
+
+@gpu
 def test_gradients_against_differences(sgemm):
     """The two gradients of combine, and of dispatch, against central differences of the forward pass (which is linear in
     each argument, so differences are exact up to rounding)."""
