@@ -158,7 +158,11 @@ __global__ void __launch_bounds__(F_THREADS, 2) mx4_few_kernel(const __grid_cons
                         for(int i = 1; i < 8; ++i)
                             dot = __hfma2(p[i], v[m][h][i], dot);
                         const float2 f = __half22float2(dot);
-                        sum[g][q][m]   = fmaf(f.x + f.y, s * sx[m][h * BLOCKS / 2], sum[g][q][m]);
+                        const float  v = f.x + f.y;
+                        const float  other = sx[m][h * BLOCKS / 2];
+                        // two mxfp4 scales can exceed FP32 together: a block that adds nothing is zero then all the same, and NaN
+                        // where the short side's scale is
+                        sum[g][q][m] = fmaf(v, FMT == B200_SGEMM_NVFP4 || v != 0.f ? s * other : other, sum[g][q][m]);
                     }
                 }
             }

@@ -319,6 +319,27 @@ def test_product_over_the_whole_range_of_scales(sgemm, fmt, dtype, M, N):
 
 
 @gpu
+@pytest.mark.parametrize("M,N", [(1, 300), (300, 2), (40, 130), (300, 200)])
+def test_product_of_huge_scales_where_the_codes_are_zero(sgemm, M, N):
+    """mxfp4 scales of 2^100 and more on both sides, where one side's codes are all zero; the other blocks' sums are exact."""
+    K, r = 1088, np.random.default_rng(M)
+    sides = []
+    for side, rows in enumerate((M, N)):
+        code = r.integers(0, 16, (rows, K)).astype(np.uint8)
+        byte = r.choice([227, 240, 252], (rows, K // 32)).astype(np.uint8)
+        block = np.arange(K // 32) % 4
+        code[:, np.repeat(block == side, 32)] = 0  # block % 4: 0 and 1 zero on one side, 2 on both, 3 on neither
+        code[:, np.repeat(block == 2, 32)] = 0
+        byte[:, block == 3] = 127
+        sides.append((*(dev(v) for v in ref.pack(ref.MXFP4, code, byte)), ref.values(ref.MXFP4, code, byte)))
+    a, b = sides
+    c = torch.empty(M, N, device="cuda")
+    sgemm.gemm_mx4(ref.MXFP4, 0, pkg.m_type.f32, c, a[0], a[1], b[0], b[1], M, N, K)
+    assert np.array_equal(c.cpu().numpy(), (a[2] @ b[2].T).astype(np.float32))
+    assert sgemm.mx4_device_status() == 0
+
+
+@gpu
 @pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_product_many_tiles(sgemm, fmt, dtype):
@@ -385,6 +406,22 @@ def test_product_of_nan_blocks_is_nan(sgemm, fmt, other):
     for nan in (torch.isnan(c), torch.isnan(t.T)):
         assert nan[7].all() and nan[39].all()
         assert nan.sum().item() == 2 * N
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
+@pytest.mark.parametrize("few", [1, 2, 3])
+def test_product_of_nan_blocks_of_the_short_side(sgemm, fmt, few):
+    M, N, K = few, 300, 1100
+    x = torch.randn(M, K)
+    x[M - 1, 777] = float("nan")
+    a = quantize(sgemm, fmt, x.cuda(), M, K, "f32")
+    b = operand(fmt, N, K, 5)
+    c, t = torch.zeros(M, N, device="cuda"), torch.zeros(N, M, device="cuda")
+    sgemm.gemm_mx4(fmt, 0, pkg.m_type.f32, c, a[0], a[1], b[0], b[1], M, N, K)
+    sgemm.gemm_mx4(fmt, 0, pkg.m_type.f32, t, b[0], b[1], a[0], a[1], N, M, K)
+    for nan in (torch.isnan(c), torch.isnan(t.T)):
+        assert nan[M - 1].all() and nan.sum().item() == N
 
 
 def grouped_case(fmt, counts, N, K, rows=None, seed=0):
