@@ -332,8 +332,9 @@ int b200_sgemm_mx4_dequantize(int format, int type, const void* codes, const voi
                               const float* global_scale, void* X, size_t ldx, void* cuda_stream);
 
 /* C[m, n] = alpha * global_a * global_b * sum_k A[m, k] B[n, k] from two quantised matrices of the same format, A of M and
- * B of N rows of K.  C is of `type_c`, row-major (ldc >= N) or col-major (ldc >= M; 0 = packed), overwritten, and overlaps no operand.  Sums are kept
- * in FP32 and rounded to type_c once.  global_a / global_b: one device float each or NULL (1); NULL for MXFP4.  A few rows on
+ * B of N rows of K.  C is of `type_c`, row-major (ldc >= N) or col-major (ldc >= M; 0 = packed), overwritten, and overlaps no
+ * operand.  Sums are kept in FP32, multiplied by the factor alpha * global_a * global_b, itself formed in FP32 (in either order:
+ * keep its parts within 2^+-126), and rounded to type_c once.  global_a / global_b: one device float each or NULL (1); NULL for MXFP4.  A few rows on
  * one side (the tokens of a decode step) are a case of its own: the long matrix streams through at the memory's rate. */
 int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, const void* a_codes, const void* a_scales, const void* b_codes,
                    const void* b_scales, size_t M, size_t N, size_t K, size_t ldc, float alpha, const float* global_a,
@@ -369,7 +370,8 @@ int b200_sgemm_route_sort(const int* expert_ids, size_t tokens, size_t top_k, si
                           int* counts, int* slot_row, int* row_slot, size_t rows, void* cuda_stream);
 
 /* Xs[slot_row[t * top_k + j]] = X[t]: X tokens x width, Xs rows x width, row-major, ldx / lds >= width (0 = packed), same
- * type.  Rows that no slot names are left as they were.  A slot_row outside 0 .. rows-1 counts as dropped, here and below. */
+ * type.  Rows that no slot names are left as they were.  A slot_row outside 0 .. rows-1 counts as dropped, here and below; where a
+ * row is written, no two slots name the same one (route_sort gives each a row of its own). */
 int b200_sgemm_route_dispatch(int type, const void* X, size_t tokens, size_t width, size_t ldx, const int* slot_row, size_t top_k,
                               void* Xs, size_t rows, size_t lds, void* cuda_stream);
 

@@ -504,7 +504,10 @@ extern "C" int b200_sgemm_route_sort(const int* expert_ids, size_t tokens, size_
     const size_t smem = (size_t)a.warps * experts * sizeof(int);
     if(smem > 48 * 1024 - sizeof(int) * (2 * MAX_EXPERTS + SORT_WARPS)) // beyond what every kernel may have
     {
-        const cudaError_t e = cudaFuncSetAttribute(route_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // always the most that a call can need: with this call's own size another thread's smaller one could take it back
+        // between here and the launch
+        constexpr int     most = SORT_WARPS * MAX_EXPERTS * (int)sizeof(int);
+        const cudaError_t e    = cudaFuncSetAttribute(route_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if(e != cudaSuccess)
             return (int)e;
     }

@@ -1,4 +1,6 @@
 """Routing (b200_sgemm_route_*): slots sorted by expert, rows there and back, and their gradients, against 64-bit numpy."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 
@@ -97,6 +99,32 @@ def test_sort_all_to_one_and_none(sgemm):
     for ids in (np.full((6000, 3), 4, np.int32), np.full((300, 2), -1, np.int32), np.full((5, 2), 2 ** 31 - 1, np.int32)):
         got, rows = run_sort(sgemm, ids, 9, 128)
         for g, w in zip(got, sort_reference(ids, 9, 128, rows)):
+            assert np.array_equal(g.cpu().numpy(), w)
+
+
+@gpu
+def test_sort_from_several_threads(sgemm):
+    """Calls that need different amounts of shared memory, at once from four threads on streams of their own."""
+    r = np.random.default_rng(5)
+    cases = []
+    for experts in (1024, 450, 700, 3):
+        ids = r.integers(0, experts, (16384, 2)).astype(np.int32)
+        out, rows = run_sort(sgemm, ids, experts, 8)
+        cases.append((dev(ids), experts, out, rows, sort_reference(ids, experts, 8, rows), torch.cuda.Stream()))
+        for o in out:
+            o.fill_(99)
+    torch.cuda.synchronize()
+
+    def work(ids, experts, out, rows, want, stream):
+        for _ in range(500):
+            sgemm.route_sort(ids, 16384, 2, experts, 8, *out, rows, stream=stream)
+
+    with ThreadPoolExecutor(len(cases)) as pool:
+        for done in [pool.submit(work, *c) for c in cases]:
+            done.result()
+    torch.cuda.synchronize()
+    for _, _, out, _, want, _ in cases:
+        for g, w in zip(out, want):
             assert np.array_equal(g.cpu().numpy(), w)
 
 
