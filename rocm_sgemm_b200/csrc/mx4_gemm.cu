@@ -85,7 +85,9 @@ struct GLayout
     static constexpr int    BY_SMEM     = (216 * 1024) / STAGE_BYTES;
     static constexpr int    BY_TMEM     = (G_TMEM_COLS - G_SCALE_COL) / SLOT_COLS;
     static constexpr int    STAGES      = BY_SMEM < BY_TMEM ? (BY_SMEM < 8 ? BY_SMEM : 8) : (BY_TMEM < 8 ? BY_TMEM : 8);
-    static constexpr int    ACCS        = BN > 128 ? 1 : 2; // accumulators
+    // accumulators.  One of 256 columns beats two of 192 for pairs, whose tiles read a fifth more bytes a product: 8192 cube 195 us
+    // against 243, experts of about 1024 rows x 4096 x 2048 130 against 152
+    static constexpr int    ACCS        = BN > 128 ? 1 : 2;
     static constexpr int    BARRIERS    = 2 * STAGES + 6;
     static constexpr size_t SMEM_BYTES  = size_t(STAGES) * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers, misc*/;
     static_assert(8 * BARRIERS + 16 <= 256 && BARRIERS <= 32, "barrier area, a lane each");
