@@ -14,7 +14,8 @@
 //   * the codes, g with at most 12 significant bits (1.0, powers of two): s g is exact in 16 bits and every midpoint t s g an
 //     FP32 number, which the next FP32 number x is so far from that the quotient in FP32 (one product and two fused
 //     multiply-adds, off by 2^-45 before its rounding) is t only if x / (s g) is: the closest case, t = 1/4 and s g just below a
-//     power of two, leaves 2^-40.
+//     power of two, leaves 2^-40.  A block with the largest scale, the only one whose x / (s g) can leave FP32's range, goes the
+//     other way, where a product may become infinite: here the fused multiply-adds would take infinities from each other.
 //   * any other g: products with the reciprocal, made a little too small and a little too large (2^-21, five roundings of
 //     2^-24 lie in between), bracket the quotient.  Where their codes differ the value is read again and the sign of
 //     |x| - (t s) g decides, exact as above.  That is rare for random g, but g = amax / 2688 of BF16 data makes every
@@ -37,6 +38,7 @@ static_assert(Q_ROWS == 32, "the rows of a CTA lie 16 bytes apart in a scale til
 constexpr int Q_COL_K   = 128;           // k of one CTA when the rows are the contiguous dimension
 
 constexpr unsigned INF_BITS  = 0x7F800000u;
+constexpr unsigned MAX_E4M3  = 0x7Eu; // 448
 
 // the matrix's scale, as every thread needs it
 struct Global
@@ -68,7 +70,7 @@ __device__ __forceinline__ Scale scale_nvfp4(unsigned amax_bits, const Global& G
     // amax - 6 m g for the midpoints m above and below c (half a step on in the bits)
     const float above = fmaf(-(__uint_as_float((2 * c + 1) << 19) * (6.f * 0x1p120f)), G.g, amax);
     const float below = fmaf(-(__uint_as_float((2 * c - 1) << 19) * (6.f * 0x1p120f)), G.g, amax);
-    if(c < 0x7Eu && (above > 0.f || (above == 0.f && (c & 1u))))
+    if(c < MAX_E4M3 && (above > 0.f || (above == 0.f && (c & 1u))))
         ++c;
     else if(c > 0u && (below < 0.f || (below == 0.f && (c & 1u))))
         --c;
@@ -177,7 +179,7 @@ __device__ __forceinline__ uint2 encode(const float (&x)[Q_LANE_K], const Scale&
         scaled16(y, x, sc.inv);
         return codes16(y);
     }
-    if(G.few)
+    if(G.few && sc.byte != MAX_E4M3)
     {
 #pragma unroll
         for(int i = 0; i < Q_LANE_K; ++i)
