@@ -114,7 +114,9 @@ __global__ void __launch_bounds__(F_THREADS, 2) mx4_few_kernel(const __grid_cons
     {
         const size_t tile = (size_t)(k / BLOCK / 4) * MX4_TILE_BYTES;
         const int    in   = k / BLOCK % 4 * 8;
-        float   sx[FEW][BLOCKS]; // of the short side, times 2^100 of the 2^120 that raw_scale lacks (448 x 2^120 is no FP32 number)
+        // scales of the short side.  nvfp4: times 2^100 of the 2^120 that raw_scale lacks (448 x 2^120 is no FP32 number).  mxfp4: a
+        // quarter, the smallest |v| but zero, so that the product of two scales only exceeds FP32 where the block's sum does
+        float   sx[FEW][BLOCKS];
         __half2 v[FEW][2][8];
 #pragma unroll
         for(int m = 0; m < FEW; ++m)
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) mx4_few_kernel(const __grid_cons
             const unsigned s = __ldg(reinterpret_cast<const unsigned*>(scales_x + tile + m * 16)) >> in;
 #pragma unroll
             for(int b = 0; b < BLOCKS; ++b)
-                sx[m][b] = scale_value<FMT>(s >> (8 * b) & 0xFFu) * (FMT == B200_SGEMM_NVFP4 ? 0x1p100f : 1.f);
+                sx[m][b] = scale_value<FMT>(s >> (8 * b) & 0xFFu) * (FMT == B200_SGEMM_NVFP4 ? 0x1p100f : 0.25f);
             pairs16(v[m][0], x.x, x.y);
             pairs16(v[m][1], x.z, x.w);
         }
@@ -160,8 +162,8 @@ __global__ void __launch_bounds__(F_THREADS, 2) mx4_few_kernel(const __grid_cons
                         const float2 f = __half22float2(dot);
                         const float  v = f.x + f.y;
                         const float  other = sx[m][h * BLOCKS / 2];
-                        // two mxfp4 scales can exceed FP32 together: a block that adds nothing is zero then all the same, and NaN
-                        // where the short side's scale is
+                        // where two mxfp4 scales exceed FP32 all the same, a block that adds nothing is zero, and NaN where the
+                        // short side's scale is
                         sum[g][q][m] = fmaf(v, FMT == B200_SGEMM_NVFP4 || v != 0.f ? s * other : other, sum[g][q][m]);
                     }
                 }
@@ -202,8 +204,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) mx4_few_kernel(const __grid_cons
         total += part[warp + i][lane];
     if(row >= a.f.rows)
         return;
-    if(FMT == B200_SGEMM_NVFP4)
-        total *= 0x1p20f;
+    total *= FMT == B200_SGEMM_NVFP4 ? 0x1p20f : 4.f;
     float factor = a.f.alpha;
     if(a.f.global_x)
         factor *= *a.f.global_x;

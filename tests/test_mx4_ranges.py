@@ -41,3 +41,40 @@ def test_quantize_saturates_with_the_sign(sgemm, g, dtype, layout):
     codes, scales = quantize(sgemm, ref.NVFP4, (x if layout == 0 else x.T).contiguous().cuda(), rows, K, dtype, layout, gt)
     assert np.array_equal(scales.cpu().numpy(), want[1])
     assert np.array_equal(codes.cpu().numpy(), want[0])
+
+
+@gpu
+@pytest.mark.parametrize("M,N", [(1, 300), (2, 129), (300, 1), (40, 130), (300, 200)])
+def test_product_of_scales_that_exceed_fp32_together(sgemm, M, N):
+    """mxfp4 blocks whose scales make 2^128 or 2^129 and whose codes make 1/4: 2^126 and 2^127, which FP32 holds, and every
+    sum of which it holds."""
+    K = 1056
+    sides = []
+    for side, rows in enumerate((M, N)):
+        code = np.zeros((rows, K), np.uint8)
+        code[:, ::32] = 1  # 0.5 once in each block
+        code[:, 32::64] |= 8 * side  # and a product of -1/4 in every other one
+        code[:, 128:] *= side  # four blocks count
+        byte = np.full((rows, K // 32), 127 + 64, np.uint8)
+        byte[:, 2] += 1 - side  # 2^126 - 2^126 + 2^127 - 2^126
+        sides.append((*(dev(v) for v in ref.pack(ref.MXFP4, code, byte)), ref.values(ref.MXFP4, code, byte)))
+    a, b = sides
+    want = a[2] @ b[2].T
+    assert (want == 2.0 ** 126).all()
+    c = torch.empty(M, N, device="cuda")
+    sgemm.gemm_mx4(ref.MXFP4, 0, pkg.m_type.f32, c, a[0], a[1], b[0], b[1], M, N, K)
+    assert np.array_equal(c.cpu().numpy(), want.astype(np.float32))
+    assert sgemm.mx4_device_status() == 0
+
+
+def repeated(fmt, rows, period, repeats, seed):
+    """A quantised matrix of positive values whose K is one period over and over, and the float64 values of a period."""
+    r = np.random.default_rng(seed)
+    code = r.integers(1, 8, (rows, period)).astype(np.uint8)
+    blocks = period // ref.BLOCK[fmt]
+    byte = (r.integers(0x30, 0x40, (rows, blocks)) if fmt == ref.NVFP4 else r.integers(124, 128, (rows, blocks))).astype(np.uint8)
+    codes, scales = ref.pack(fmt, code, byte)
+    codes = dev(codes).view(rows, -1).repeat(1, repeats)
+    bands = -(-rows // 128)
+    scales = dev(scales).view(bands, -1).repeat(1, repeats)
+    return codes.view(-1), scales.view(-1), ref.values(fmt, code, byte)
