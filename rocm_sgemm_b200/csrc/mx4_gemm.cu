@@ -17,8 +17,9 @@
 //   warps 0-7  accumulate and store.  The tensor core adds into its FP32 accumulator with truncation, so for an FP32
 //              result the accumulator is emptied into registers every 1024 or 2048 k and the parts are added there,
 //              rounded to nearest (relative error of the whole result with operands of a wide range, K = 16384: 1.2e-7 in parts
-//              of 256 k, 2.9e-7 of 1024, 5.3e-7 of 2048; an FP32 product on the FMA pipe 2.4e-7); results of 16 bits keep one
-//              accumulator for the whole of K (a bias of at most 2^-23 a product of 64 k, below their rounding up to K = 2^18).
+//              of 256 k, 2.9e-7 of 1024, 5.3e-7 of 2048; an FP32 product on the FMA pipe 2.4e-7).  A bias of at most 2^-23 a
+//              product of 64 k: it stays below a quarter of the smallest rounding of an FP16 result (2^-12) up to 2^15 k and of
+//              a BF16 one (2^-9) up to 2^18, so those keep one accumulator that long and empty it as FP32 results do beyond.
 //   warp 8     fetches the stages by TMA: the two operands' codes (256 k = rows of 128 bytes, 128-byte swizzle) and the scale
 //              tiles as they lie; zero beyond the matrix
 //   warp 9     copies the stage's scale tiles into tensor memory (tcgen05.cp, replicated to the four lane quarters) and issues
@@ -54,7 +55,8 @@ constexpr int G_MAX_GROUPS = 1024;
 constexpr int MAX_SPLIT    = 8; // CTAs that share a tile's K
 constexpr int CHUNK_F32    = 4; // K blocks (1024 k, 16 products) added inside the tensor core for an FP32 result
 constexpr int CHUNK_F32_WIDE = 8; // the same for 256 columns, whose one accumulator stands still while it is emptied
-// Registers of the kernel that keeps 128 FP32 sums a thread: 12 warps are launched with 168 each; warps 8 to 11 give theirs up
+constexpr int CHUNK_F16    = 1 << 7, CHUNK_BF16 = 1 << 10; // 2^15 and 2^18 k
+// Registers of the kernel that keeps 128 sums a thread: 12 warps are launched with 168 each; warps 8 to 11 give theirs up
 // and warps 0 to 7 take them: 256 x 224 + 128 x 56 = 384 x 168, exactly the launch's allocation, so the increase is always granted.
 constexpr int G_LAUNCH_REGS = 168, G_SUM_REGS = 224, G_ISSUE_REGS = 56;
 static_assert(G_EPILOGUE * G_SUM_REGS + 128 * G_ISSUE_REGS == (G_EPILOGUE + 128) * G_LAUNCH_REGS, "register budgets");
@@ -65,7 +67,7 @@ constexpr int G_ERR_GROUP = 2; // a group's offset or count does not fit the mat
 __device__ int g_mx4_status;
 
 // PAIR: CTAs that share a tile's instructions
-// SUMS: 256 columns of FP32 results, added in registers
+// SUMS: 256 columns of results whose parts are added in registers
 template<int FMT, int BN, int PAIR, bool SUMS = false>
 struct GLayout
 {
@@ -681,7 +683,7 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1)
         {
             const Tile t = tile_at<BN, L::TILE_P>(a, first_tile, tile);
             const float factor = a.global_p ? factor_q * a.global_p[t.group] : factor_q; // fetched while the tile is computed
-            if constexpr(L::ACCS == 1 && !SUMS) // results of 16 bits: rounded into registers, so that the one accumulator is free at once
+            if constexpr(L::ACCS == 1 && !SUMS) // 16 bits, all of K: rounded into registers, so that the one accumulator is free at once
             {
                 uint32_t    out[COLS / 2];
                 if(!warp_wait(acc_full(0), acc_ph, abort_flag)) { fail(3); ok = false; break; }
@@ -768,12 +770,7 @@ __global__ void __launch_bounds__(GLayout<FMT, BN, PAIR, SUMS>::THREADS, 1)
                     break;
                 const int p = lane0 + quarter * 32 + lane, q = half * COLS;
                 if(PAIR > 1 || split == 1)
-                {
-                    if constexpr(SUMS)
-                        store_columns<float>(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
-                    else
-                        store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
-                }
+                    store_typed(a, acc, factor, t.p0 + p, t.q0 + q, t.q_end);
                 else // park the part in the ring, which is at rest: a CTA of a split tile has no other
                 {
                     float* parked = reinterpret_cast<float*>(ring);
@@ -961,19 +958,19 @@ struct Cut
 // The cut with the least estimated time, from what two dozen shapes between 100 x 1000 x 300 and 2560^3 measured (us): a K block
 // takes 0.33 / 0.37 / 0.37 in tiles of 64 / 128 / 256 columns, for the SMs go through it at about the same pace whatever
 // its width; storing a tile 1.1 / 1.75 / 2.3 where the next tile's blocks do not hide it, and 0.4 / 0.9 / 2 more at the end; FP32
-// results in 256 columns, which are added in registers, 0.4 a block, 3.7 and 3.5; adding the parts of a split tile 2.2 / 3.3.
+// results (and any whose parts are added) in 256 columns 0.4 a block, 3.7 and 3.5; adding the parts of a split tile 2.2 / 3.3.
 // Examples, us for (columns, split), BF16: 2048^3 (128, 1) 11.5, (256, 1) 9.1; 64 x 8192 x 8192 (64, 1) 13.9, (64, 2) 12.1,
 // (128, 2) 12.9; 512 x 512 x 8192 (64, 1) 13.5, (64, 4) 9.7; 512^3 (64, 1) 4.7, (64, 2) 7.0, (128, 1) 5.4.
 // lane_rows, column_rows: extents of one group; clusters of 8 and 4 CTAs do not fill every part of the chip, so they are held
 // below three quarters and seven eighths of the SMs.
-Cut cut_of(size_t lane_rows, size_t column_rows, size_t groups, int kblocks, bool f32, bool may_split, int sms)
+Cut cut_of(size_t lane_rows, size_t column_rows, size_t groups, int kblocks, bool in_parts, bool may_split, int sms)
 {
     Cut   best = {64, 1};
     float least = 1e30f;
     for(int i = 0; i < 3; ++i)
     {
         const int    columns = 64 << i, lanes = i == 2 ? 256 : 128, slots = i == 2 ? sms / 2 : sms;
-        const bool   sums  = f32 && i == 2;
+        const bool   sums  = in_parts && i == 2;
         const float  block = i == 0 ? 0.33f : (sums ? 0.4f : 0.37f), join = i == 0 ? 2.2f : 3.3f;
         const float  store = i == 0 ? 1.1f : (i == 1 ? 1.75f : (sums ? 3.7f : 2.3f));
         const float  end   = i == 0 ? 0.4f : (i == 1 ? 0.9f : (sums ? 3.5f : 2.f));
@@ -1060,8 +1057,8 @@ template<int FMT>
 int launch_tile(int columns, const GArgs& a, const Operand& p, const Operand& q, int device, int sms, cudaStream_t stream)
 {
     if(columns == 256)
-        return a.type == B200_SGEMM_F32 ? launch<FMT, 256, 2, true>(a, p, q, device, sms, stream)
-                                        : launch<FMT, 256, 2>(a, p, q, device, sms, stream);
+        return a.type == B200_SGEMM_F32 || a.chunk < a.kblocks ? launch<FMT, 256, 2, true>(a, p, q, device, sms, stream)
+                                                                : launch<FMT, 256, 2>(a, p, q, device, sms, stream);
     return columns == 64 ? launch<FMT, 64, 1>(a, p, q, device, sms, stream) : launch<FMT, 128, 1>(a, p, q, device, sms, stream);
 }
 
@@ -1074,10 +1071,12 @@ int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_
     a.K           = (int)K;
     a.kblocks     = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
     a.bands_p     = (a.np + MX4_BAND - 1) / MX4_BAND;
-    const Cut cut = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, a.type == B200_SGEMM_F32, a.groups == 0, sms);
+    const int  most     = a.type == B200_SGEMM_F16 ? CHUNK_F16 : CHUNK_BF16; // K blocks in one accumulator of a 16-bit result
+    const bool in_parts = a.type == B200_SGEMM_F32 || a.kblocks > most;
+    const Cut  cut      = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, in_parts, a.groups == 0, sms);
     while((1 << a.split_bits) < cut.split)
         ++a.split_bits;
-    a.chunk       = a.type != B200_SGEMM_F32 ? a.kblocks : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
+    a.chunk = a.type != B200_SGEMM_F32 ? (in_parts ? most : a.kblocks) : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
     return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(cut.columns, a, p, q, device, sms, stream)
                                       : launch_tile<B200_SGEMM_MXFP4>(cut.columns, a, p, q, device, sms, stream);
 }

@@ -78,3 +78,51 @@ def repeated(fmt, rows, period, repeats, seed):
     bands = -(-rows // 128)
     scales = dev(scales).view(bands, -1).repeat(1, repeats)
     return codes.view(-1), scales.view(-1), ref.values(fmt, code, byte)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
+@pytest.mark.parametrize("dtype,K", [("f16", 1 << 24), ("bf16", 1 << 27)])
+def test_long_sums_of_one_sign(sgemm, fmt, dtype, K):
+    """The tensor core cuts off where it adds (2^-22 of the sum for each of its 64 k): 16-bit results too have to leave it
+    before that shows.  One accumulator holds 2^15 k for FP16 and 2^18 for BF16, 2^9 and 2^12 of its steps; the parts, and
+    the sums of up to eight CTAs, are added with 2^-24 each."""
+    M, N, period = 3, 5, 4096
+    a, b = repeated(fmt, M, period, K // period, 1), repeated(fmt, N, period, K // period, 2)
+    want = a[2] @ b[2].T * (K // period)
+    alpha = 2.0 ** -np.floor(np.log2(want.max()))
+    c = torch.empty(M, N, dtype=TYPES[dtype], device="cuda")
+    sgemm.gemm_mx4(fmt, 0, pkg.m_type[dtype], c, a[0], a[1], b[0], b[1], M, N, K, alpha=float(alpha))
+    want = want * alpha
+    held = 15 if dtype == "f16" else 18
+    bound = 2.0 ** (held - 6 - 22) + (K / 2.0 ** held + 8) * 2.0 ** -24 + ref.TYPE_EPS[dtype] / 2 + 4 * 2.0 ** -24
+    off = np.abs(c.double().cpu().numpy() - want) / want
+    assert off.max() <= bound, f"{off.max() / bound:.3g} times the bound"
+    assert sgemm.mx4_device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS, ids=fmt_ids)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("layout_c", [0, 1])
+def test_long_sums_in_wide_tiles(sgemm, fmt, dtype, layout_c):
+    """K beyond what one accumulator may hold of FP16, in tiles of 256 columns."""
+    M, N, period, repeats = 2304, 2560, 1024, 33
+    K = period * repeats
+    assert sgemm.mx4_sizes(fmt, M, K)[0] == M * K // 2
+    a, b = repeated(fmt, M, period, repeats, 3), repeated(fmt, N, period, repeats, 4)
+    va, vb = torch.from_numpy(a[2]).cuda(), torch.from_numpy(b[2]).cuda()
+    want = (va @ vb.T * repeats).cpu().numpy()
+    alpha = float(2.0 ** -np.floor(np.log2(want.max())))
+    ld = (N if layout_c == 0 else M) + 8
+    c = torch.full((M if layout_c == 0 else N, ld), 9.0, dtype=TYPES[dtype], device="cuda")
+    sgemm.gemm_mx4(fmt, layout_c, pkg.m_type[dtype], c, a[0], a[1], b[0], b[1], M, N, K, ldc=ld, alpha=alpha)
+    assert (c[:, ld - 8:] == 9).all()
+    got = c[:, :ld - 8].double().cpu().numpy()
+    got = got if layout_c == 0 else got.T
+    held = {"f32": 11, "f16": 15, "bf16": 18}[dtype]
+    steps = min(2.0 ** held, K) / 64
+    bound = steps * 2.0 ** -22 + (K / 2.0 ** held + 8) * 2.0 ** -24 + ref.TYPE_EPS[dtype] / 2 + 4 * 2.0 ** -24
+    off = np.abs(got - want * alpha) / (want * alpha)
+    assert off.max() <= bound, f"{off.max() / bound:.3g} times the bound"
+    assert sgemm.mx4_device_status() == 0
