@@ -316,8 +316,8 @@ size_t b200_sgemm_mx4_scale_bytes(int format, size_t rows, size_t K);
  *   NVFP4  s = RN_e4m3(amax / (6 g)), at most 448;    code = RN_e2m1(x / (s g)), at most 6; g = *global_scale, 1 if NULL
  *   MXFP4  s = 2^(floor(log2 amax) - 2), in 2^+-127;  code = RN_e2m1(x / s), at most 6; global_scale has to be NULL
  * with amax the block's largest magnitude.  s = 0 gives zero codes.  A block with an infinity or a NaN has the NaN scale
- * (0x7F, 0xFF) and zero codes; a g that is not in 2^-90 .. 2^90 gives NaN scales everywhere.  The values that stand
- * for X are code * s * g.
+ * (0x7F, 0xFF) and zero codes; so has every block where g is not in 2^-90 .. 2^90, but that blocks of zeros have scale 0 for
+ * any finite g >= 0 (g = amax / 2688 of a matrix of zeros is 0).  The values that stand for X are code * s * g.
  * row_index (NULL: none; row-major X only): row r is X row row_index[r] / index_div, X has source_rows rows; a negative index
  * or one behind X leaves the codes of row r as they were and its scales zero, and a band of 128 rows without any
  * valid index is not written at all.  With the row_slot of b200_sgemm_route_sort and index_div = top_k this sorts tokens and

@@ -4,7 +4,8 @@
 // Definition, in exact arithmetic (RN = round to nearest, ties to the even code; a block is 16 or 32 neighbours along k):
 //   nvfp4   s = RN_e4m3(amax / (6 g)), at most 448;      code = RN_e2m1(x / (s g)), at most 6
 //   mxfp4   s = 2^(floor(log2 amax) - 2), in 2^+-127;    code = RN_e2m1(x / s),     at most 6
-// amax is the block's largest magnitude, g the matrix's FP32 scale.  s = 0 (nvfp4, a block far below g) gives codes 0.
+// amax is the block's largest magnitude, g the matrix's FP32 scale.  s = 0 (nvfp4, a block far below g) gives codes 0; a block
+// of zeros has s = 0 for every finite g >= 0, so that g = amax / 2688 of a matrix of zeros does.
 // A block that holds an infinity or a NaN has the NaN scale and codes 0, so whatever is computed from it is NaN.
 //
 // How the kernel stays exact without dividing in 64 bits.  mxfp4: x / s is a multiplication by a power of two.  nvfp4:
@@ -43,16 +44,18 @@ constexpr unsigned MAX_E4M3  = 0x7Eu; // 448
 // the matrix's scale, as every thread needs it
 struct Global
 {
-    float g, r6;   // 1 / (6 g)
-    bool  ok, few; // ok: finite and in 2^+-90, where none of the products below can leave FP32's range; few: <= 12 bits
+    float    g, r6; // 1 / (6 g), or 0 where g is not in 2^+-90, in which none of the products below can leave FP32's range
+    unsigned limit; // largest magnitudes from these bits on give NaN: infinity; 1 where g is not in 2^+-90, 0 where it is no scale
+    bool     few;   // g has <= 12 bits
 };
 __device__ __forceinline__ Global load_global(const float* p)
 {
     Global G;
-    G.g   = p ? *p : 1.f;
-    G.r6  = __frcp_rn(6.f * G.g);
-    G.ok  = G.g >= 0x1p-90f && G.g <= 0x1p90f;
-    G.few = (__float_as_uint(G.g) & 0xFFFu) == 0;
+    G.g = p ? *p : 1.f;
+    const bool ok = G.g >= 0x1p-90f && G.g <= 0x1p90f;
+    G.r6    = ok ? __frcp_rn(6.f * G.g) : 0.f;
+    G.limit = ok ? INF_BITS : (G.g >= 0.f && G.g < __uint_as_float(INF_BITS) ? 1u : 0u);
+    G.few   = (__float_as_uint(G.g) & 0xFFFu) == 0;
     return G;
 }
 
@@ -74,7 +77,7 @@ __device__ __forceinline__ Scale scale_nvfp4(unsigned amax_bits, const Global& G
         ++c;
     else if(c > 0u && (below < 0.f || (below == 0.f && (c & 1u))))
         --c;
-    const bool bad = amax_bits >= INF_BITS || !G.ok;
+    const bool bad = amax_bits >= G.limit;
     r.byte = bad ? NAN_E4M3 : c;
     r.s    = e4m3_value(c);
     r.sg   = r.s * G.g;

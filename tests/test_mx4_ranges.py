@@ -126,3 +126,40 @@ def test_long_sums_in_wide_tiles(sgemm, fmt, dtype, layout_c):
     off = np.abs(got - want * alpha) / (want * alpha)
     assert off.max() <= bound, f"{off.max() / bound:.3g} times the bound"
     assert sgemm.mx4_device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("g", [0.0, 2.0 ** -120, 2.0 ** 100])
+def test_zeros_stay_zero_whatever_the_matrix_scale(sgemm, dtype, layout, g):
+    """A matrix of zeros has amax / 2688 = 0 for a scale: its values are zero, not NaN, and so are its products."""
+    M, N, K = 70, 130, 100
+    gt = torch.tensor([g], dtype=torch.float32, device="cuda")
+    x = torch.zeros(M, K, dtype=TYPES[dtype], device="cuda")
+    x[3, 5] = -0.0
+    a = quantize(sgemm, ref.NVFP4, x if layout == 0 else x.T.contiguous(), M, K, dtype, layout, gt)
+    assert not a[0].any() and not a[1].any()
+    out = torch.full((M, K), 7.0, device="cuda")
+    sgemm.mx4_dequantize(ref.NVFP4, pkg.m_type.f32, *a, M, K, out, global_scale=gt)
+    assert not out.any()
+    b = quantize(sgemm, ref.NVFP4, torch.randn(N, K, device="cuda"), N, K, "f32")
+    for rows in (1, 2, M):
+        c = torch.full((rows, N), 7.0, device="cuda")
+        sgemm.gemm_mx4(ref.NVFP4, 0, pkg.m_type.f32, c, *a, *b, rows, N, K, global_a=gt)
+        assert not c.any()
+    # a value in it that is not zero makes its own block NaN and no other
+    x[7, 20] = 1.0
+    a = quantize(sgemm, ref.NVFP4, x if layout == 0 else x.T.contiguous(), M, K, dtype, layout, gt)
+    _, byte = ref.unpack(ref.NVFP4, a[0].cpu().numpy(), a[1].cpu().numpy(), M, K)
+    want = np.zeros_like(byte)
+    want[7, 1] = 0x7F
+    assert np.array_equal(byte, want) and not a[0].any()
+
+
+@gpu
+@pytest.mark.parametrize("g", [-1.0, float("nan"), float("inf"), -float("inf")])
+def test_zeros_with_a_matrix_scale_that_is_no_scale(sgemm, g):
+    a = quantize(sgemm, ref.NVFP4, torch.zeros(5, 40, device="cuda"), 5, 40, "f32", g=torch.tensor([g], device="cuda"))
+    _, byte = ref.unpack(ref.NVFP4, a[0].cpu().numpy(), a[1].cpu().numpy(), 5, 40)
+    assert (byte == 0x7F).all()
