@@ -19,6 +19,7 @@ import argparse
 import concurrent.futures as cf
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -60,6 +61,17 @@ def _digest(paths, flags) -> str:
     return h.hexdigest()[:16]
 
 
+def check_registers(source: str, log: str) -> None:
+    """Raises where ptxas gave a kernel that hands registers from warp to warp another number than its source counts on: the
+    library would leave that kernel out and take a slower one.  `log`: what nvcc -Xptxas -v printed for `source`."""
+    want = re.search(r"G_LAUNCH_REGS = (\d+)", source)
+    if not want:
+        return
+    used = re.findall(r"Compiling entry function '\w*mx4_gemm_kernelILi\dELi\d+ELi\dELb1E\w*'.*?Used (\d+) registers", log, re.S)
+    if not used or any(n != want[1] for n in used):
+        raise RuntimeError(f"mx4_gemm_kernel with sums in registers takes {used} registers, its source counts on {want[1]}")
+
+
 def _compile(src: Path, deps, flags, verbose=False, ptxas_log: Path | None = None, stem: str | None = None) -> Path:
     BUILD.mkdir(exist_ok=True)
     tag = _digest([src] + list(deps), flags)
@@ -73,6 +85,11 @@ def _compile(src: Path, deps, flags, verbose=False, ptxas_log: Path | None = Non
     r = subprocess.run(cmd, capture_output=True, text=True, env=_env())
     if r.returncode != 0:
         raise RuntimeError(f"nvcc failed for {src.name}:\n{r.stderr[-4000:]}")
+    try:
+        check_registers(src.read_text(), r.stderr)
+    except RuntimeError:
+        obj.unlink(missing_ok=True)
+        raise
     if ptxas_log is not None:
         with open(ptxas_log, "a") as f:
             f.write(f"== {src.name}\n{r.stderr}\n")

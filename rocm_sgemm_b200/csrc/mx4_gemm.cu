@@ -1033,7 +1033,7 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
             cudaFuncAttributes f;
             if(const cudaError_t e = cudaFuncGetAttributes(&f, kernel); e != cudaSuccess)
                 return (int)e;
-            if(f.numRegs != G_LAUNCH_REGS) // the registers would not add up
+            if(f.numRegs != G_LAUNCH_REGS) // the registers would not add up (the build refuses such a kernel)
                 return B200_SGEMM_NO_KERNEL;
         }
         ready.fetch_or(bit, std::memory_order_relaxed);
@@ -1056,9 +1056,14 @@ int launch(GArgs a, const Operand& p, const Operand& q, int device, int sms, cud
 template<int FMT>
 int launch_tile(int columns, const GArgs& a, const Operand& p, const Operand& q, int device, int sms, cudaStream_t stream)
 {
-    if(columns == 256)
-        return a.type == B200_SGEMM_F32 || a.chunk < a.kblocks ? launch<FMT, 256, 2, true>(a, p, q, device, sms, stream)
-                                                                : launch<FMT, 256, 2>(a, p, q, device, sms, stream);
+    if(columns == 256 && a.type != B200_SGEMM_F32 && a.chunk >= a.kblocks)
+        return launch<FMT, 256, 2>(a, p, q, device, sms, stream);
+    if(columns == 256) // a build whose registers do not add up takes narrower tiles
+    {
+        const int status = launch<FMT, 256, 2, true>(a, p, q, device, sms, stream);
+        if(status != B200_SGEMM_NO_KERNEL)
+            return status;
+    }
     return columns == 64 ? launch<FMT, 64, 1>(a, p, q, device, sms, stream) : launch<FMT, 128, 1>(a, p, q, device, sms, stream);
 }
 
