@@ -107,7 +107,7 @@ EXPORTS = ("b200_sgemm", "b200_sgemm_ex", "b200_sgemm_workspace_bytes", "b200_sg
            "b200_sgemm_blas_shutdown", "b200_sgemm_multi", "b200_sgemm_stream_plan",
            "b200_sgemm_selftest_bounded_wait", "b200_sgemm_trial", "b200_sgemm_mx4_code_bytes", "b200_sgemm_mx4_scale_bytes",
            "b200_sgemm_mx4_quantize", "b200_sgemm_mx4_dequantize", "b200_sgemm_mx4", "b200_sgemm_mx4_grouped",
-           "b200_sgemm_mx4_device_status", "b200_sgemm_route_capacity", "b200_sgemm_route_sort", "b200_sgemm_route_dispatch",
+           "b200_sgemm_mx4_plan", "b200_sgemm_mx4_device_status", "b200_sgemm_route_capacity", "b200_sgemm_route_sort", "b200_sgemm_route_dispatch",
            "b200_sgemm_route_combine", "b200_sgemm_route_combine_backward")
 
 
@@ -155,6 +155,7 @@ def lib() -> ctypes.CDLL:
             ("b200_sgemm_mx4_dequantize", [i, i, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp], i),
             ("b200_sgemm_mx4", [i, i, i] + [_vp] * 5 + [_sz] * 4 + [ctypes.c_float, _vp, _vp, _vp], i),
             ("b200_sgemm_mx4_grouped", [i, i] + [_vp] * 5 + [_sz] * 5 + [_vp, _vp, _sz, ctypes.c_float, _vp, _vp, _vp], i),
+            ("b200_sgemm_mx4_plan", [i, i] + [_sz] * 4 + [i, ip, ip], i),
             ("b200_sgemm_mx4_device_status", [ip], i),
             ("b200_sgemm_route_capacity", [_sz] * 4, _sz),
             ("b200_sgemm_route_sort", [_vp] + [_sz] * 4 + [_vp] * 4 + [_sz, _vp], i),
@@ -450,6 +451,13 @@ def gemm_mx4_grouped(fmt, dtype_c, C, A_codes, A_scales, B_codes, B_scales, rows
     _check(lib().b200_sgemm_mx4_grouped(fmt, dtype_c, _ptr(C), _ptr(A_codes), _ptr(A_scales), _ptr(B_codes), _ptr(B_scales), rows,
                                         N, K, ldc, groups, _ptr(offsets), _ptr(counts), used_rows, alpha, _ptr(global_a),
                                         _ptr(global_b), _stream(stream)))
+
+
+def mx4_plan(layout_c, dtype_c, M: int, N: int, K: int, groups: int = 0, sm_count: int = 148) -> tuple:
+    """(columns of a tile, CTAs that share a tile's K) of a 4-bit product (b200_sgemm_mx4_plan)."""
+    columns, split = ctypes.c_int(0), ctypes.c_int(0)
+    _check(lib().b200_sgemm_mx4_plan(layout_c, dtype_c, M, N, K, groups, sm_count, ctypes.byref(columns), ctypes.byref(split)))
+    return columns.value, split.value
 
 
 def mx4_device_status() -> int:

@@ -1067,21 +1067,41 @@ int launch_tile(int columns, const GArgs& a, const Operand& p, const Operand& q,
     return columns == 64 ? launch<FMT, 64, 1>(a, p, q, device, sms, stream) : launch<FMT, 128, 1>(a, p, q, device, sms, stream);
 }
 
-// `a` holds what both entries agree on; `columns` is the expected number of rows of Q in a group
+// K blocks that one accumulator of a 16-bit result may hold
+int most_blocks(int type) { return type == B200_SGEMM_F16 ? CHUNK_F16 : CHUNK_BF16; }
+int blocks_of(size_t K) { return (int)((K + G_KBLOCK - 1) / G_KBLOCK); }
+bool added_in_parts(int type, int kblocks) { return type == B200_SGEMM_F32 || kblocks > most_blocks(type); }
+
+// The cut of a product of `lanes` rows of P and `columns` of Q, or the rows of Q to be expected in one of `groups`.
+Cut cut_for(int type, size_t lanes, size_t columns, size_t groups, size_t K, int sms)
+{
+    const int kblocks = blocks_of(K);
+    return cut_of(lanes, columns, groups ? groups : 1, kblocks, added_in_parts(type, kblocks), groups == 0, sms);
+}
+// whether B takes the lanes: they are C's contiguous dimension, unless that one is short and the other is not
+bool lanes_from_b(bool row, size_t M, size_t N)
+{
+    const size_t packed = row ? N : M;
+    return packed <= 64 && (row ? M : N) > packed ? !row : row;
+}
+size_t rows_of_group(size_t rows, size_t groups) { return (rows + groups - 1) / groups; }
+
+// `a` holds what both entries agree on; `columns` as in cut_for
 int run(int format, GArgs a, const Operand& p, const Operand& q, size_t K, size_t columns, cudaStream_t stream)
 {
     int device = 0, sms = 0, status = device_sms(&device, &sms);
     if(status != B200_SGEMM_OK)
         return status;
     a.K           = (int)K;
-    a.kblocks     = (int)((K + G_KBLOCK - 1) / G_KBLOCK);
+    a.kblocks     = blocks_of(K);
     a.bands_p     = (a.np + MX4_BAND - 1) / MX4_BAND;
-    const int  most     = a.type == B200_SGEMM_F16 ? CHUNK_F16 : CHUNK_BF16; // K blocks in one accumulator of a 16-bit result
-    const bool in_parts = a.type == B200_SGEMM_F32 || a.kblocks > most;
-    const Cut  cut      = cut_of((size_t)a.np, columns, a.groups ? (size_t)a.groups : 1, a.kblocks, in_parts, a.groups == 0, sms);
+    const Cut cut = cut_for(a.type, (size_t)a.np, columns, (size_t)a.groups, K, sms);
     while((1 << a.split_bits) < cut.split)
         ++a.split_bits;
-    a.chunk = a.type != B200_SGEMM_F32 ? (in_parts ? most : a.kblocks) : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
+    if(!added_in_parts(a.type, a.kblocks))
+        a.chunk = a.kblocks;
+    else
+        a.chunk = a.type != B200_SGEMM_F32 ? most_blocks(a.type) : (cut.columns == 256 ? CHUNK_F32_WIDE : CHUNK_F32);
     return format == B200_SGEMM_NVFP4 ? launch_tile<B200_SGEMM_NVFP4>(cut.columns, a, p, q, device, sms, stream)
                                       : launch_tile<B200_SGEMM_MXFP4>(cut.columns, a, p, q, device, sms, stream);
 }
@@ -1130,10 +1150,7 @@ extern "C" int b200_sgemm_mx4(int format, int layout_c, int type_c, void* C, con
         f.type     = type_c;
         return mx4_few(format, f, sms, static_cast<cudaStream_t>(cuda_stream));
     }
-    // lanes: C's contiguous dimension, unless that one is short and the other is not
-    bool b_lanes = row;
-    if(packed <= 64 && (row ? M : N) > packed)
-        b_lanes = !row;
+    const bool b_lanes = lanes_from_b(row, M, N);
     GArgs g     = {};
     g.c         = C;
     g.sp        = b_lanes == row ? 1 : (long long)ldc;
@@ -1181,7 +1198,28 @@ extern "C" int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const voi
     const size_t used = used_rows && used_rows < rows ? used_rows : rows;
     const Operand b{b_codes, b_scales, groups * N, groups * ((N + MX4_BAND - 1) / MX4_BAND)};
     const Operand a{a_codes, a_scales, rows, (rows + MX4_BAND - 1) / MX4_BAND};
-    return run(format, g, b, a, K, (used + groups - 1) / groups, static_cast<cudaStream_t>(cuda_stream));
+    return run(format, g, b, a, K, rows_of_group(used, groups), static_cast<cudaStream_t>(cuda_stream));
+}
+
+extern "C" int b200_sgemm_mx4_plan(int layout_c, int type_c, size_t M, size_t N, size_t K, size_t groups, int sm_count, int* columns,
+                                   int* split)
+{
+    if(!columns || !split || M == 0 || N == 0 || K == 0 || !type_ok(type_c) || layout_c & ~1 || sm_count < 1
+       || (groups && layout_c != B200_SGEMM_ROW_MAJOR))
+        return B200_SGEMM_INVALID_ARGUMENT;
+    if(M > MAX_EXTENT || N > MAX_EXTENT || K > MAX_EXTENT || groups > G_MAX_GROUPS || groups * N > MAX_EXTENT)
+        return B200_SGEMM_UNSUPPORTED_SIZE;
+    if(groups == 0 && mx4_is_few(M < N ? M : N, M < N ? N : M, K))
+    {
+        *columns = 0;
+        *split   = 1;
+        return B200_SGEMM_OK;
+    }
+    const bool b_lanes = groups || lanes_from_b(layout_c == B200_SGEMM_ROW_MAJOR, M, N);
+    const Cut  cut     = cut_for(type_c, b_lanes ? N : M, groups ? rows_of_group(M, groups) : (b_lanes ? M : N), groups, K, sm_count);
+    *columns = cut.columns;
+    *split   = cut.split;
+    return B200_SGEMM_OK;
 }
 
 extern "C" int b200_sgemm_mx4_device_status(int* status)
