@@ -97,6 +97,18 @@ __device__ __forceinline__ float scale_value(unsigned byte)
     return byte == NAN_E8M0 ? nan : e8m0_value(byte);
 }
 
+// Launches a kernel and returns this launch's own status; cudaPeekAtLastError would also give what an earlier call that failed
+// (an allocation that another entry did not get) left behind.
+template<class Args>
+int launch_kernel(void (*kernel)(Args), unsigned grid, int threads, cudaStream_t stream, const Args& a)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim            = dim3(grid);
+    cfg.blockDim           = dim3((unsigned)threads);
+    cfg.stream             = stream;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 // f(type as a C++ type) for a checked element type
 template<class F>
 int with_type(int type, F f)

@@ -223,11 +223,7 @@ __global__ void __launch_bounds__(F_THREADS, 2) mx4_few_kernel(const __grid_cons
 template<int FMT>
 int launch(const Args& a, unsigned grid, cudaStream_t stream)
 {
-    if(a.f.few == 1)
-        mx4_few_kernel<FMT, 1><<<grid, F_THREADS, 0, stream>>>(a);
-    else
-        mx4_few_kernel<FMT, 2><<<grid, F_THREADS, 0, stream>>>(a);
-    return (int)cudaPeekAtLastError();
+    return launch_kernel(a.f.few == 1 ? mx4_few_kernel<FMT, 1> : mx4_few_kernel<FMT, 2>, grid, F_THREADS, stream, a);
 }
 } // namespace
 

@@ -603,21 +603,10 @@ extern "C" int b200_sgemm_mx4_quantize(int format, int layout, int type, const v
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        if(row_major)
-        {
-            if(format == B200_SGEMM_NVFP4)
-                quantize_rows_kernel<B200_SGEMM_NVFP4, T><<<grid, Q_THREADS, 0, stream>>>(a);
-            else
-                quantize_rows_kernel<B200_SGEMM_MXFP4, T><<<grid, Q_THREADS, 0, stream>>>(a);
-        }
-        else
-        {
-            if(format == B200_SGEMM_NVFP4)
-                quantize_cols_kernel<B200_SGEMM_NVFP4, T><<<grid, Q_THREADS, 0, stream>>>(a);
-            else
-                quantize_cols_kernel<B200_SGEMM_MXFP4, T><<<grid, Q_THREADS, 0, stream>>>(a);
-        }
-        return (int)cudaPeekAtLastError();
+        const bool nv = format == B200_SGEMM_NVFP4;
+        auto kernel = row_major ? (nv ? quantize_rows_kernel<B200_SGEMM_NVFP4, T> : quantize_rows_kernel<B200_SGEMM_MXFP4, T>)
+                                : (nv ? quantize_cols_kernel<B200_SGEMM_NVFP4, T> : quantize_cols_kernel<B200_SGEMM_MXFP4, T>);
+        return launch_kernel(kernel, grid, Q_THREADS, stream, a);
     });
 }
 
@@ -657,7 +646,6 @@ extern "C" int b200_sgemm_mx4_dequantize(int format, int type, const void* codes
         };
         auto kernel = format == B200_SGEMM_NVFP4 ? pick(std::integral_constant<int, B200_SGEMM_NVFP4>())
                                                  : pick(std::integral_constant<int, B200_SGEMM_MXFP4>());
-        kernel<<<grid, Q_THREADS, 0, stream>>>(a);
-        return (int)cudaPeekAtLastError();
+        return launch_kernel(kernel, grid, Q_THREADS, stream, a);
     });
 }

@@ -449,7 +449,7 @@ unsigned warp_grid(const RowArgs& a, int* pieces, int n, int unroll)
     const size_t ctas = ((size_t)a.tokens * *pieces + R_THREADS / 32 - 1) / (R_THREADS / 32);
     return ctas > 0x7fffffffull ? 0u : (unsigned)ctas;
 }
-// launches f(grid, many) for the two ways of taking a row: `many` from one wave of 148 SMs x 8 CTAs on
+// f(grid, many), which launches, for the two ways of taking a row: `many` from one wave of 148 SMs x 8 CTAs on
 template<class F>
 int with_grid(RowArgs& a, int n, F f)
 {
@@ -459,8 +459,7 @@ int with_grid(RowArgs& a, int n, F f)
         grid = warp_grid(a, &a.pieces, n, 1);
     if(!grid)
         return B200_SGEMM_UNSUPPORTED_SIZE;
-    f(grid, many);
-    return (int)cudaPeekAtLastError();
+    return f(grid, many);
 }
 } // namespace
 
@@ -552,7 +551,7 @@ extern "C" int b200_sgemm_route_dispatch(int type, const void* X, size_t tokens,
     return with_pieces(type, rows_vector(type, X, ldx) && rows_vector(type, Xs, lds), width, [&](auto t, auto n) {
         return with_grid(a, n(), [&](unsigned grid, bool many) {
             auto kernel = many ? route_dispatch_kernel<decltype(t), n(), 4> : route_dispatch_kernel<decltype(t), n(), 1>;
-            kernel<<<grid, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
+            return launch_kernel(kernel, grid, R_THREADS, static_cast<cudaStream_t>(cuda_stream), a);
         });
     });
 }
@@ -585,7 +584,7 @@ extern "C" int b200_sgemm_route_combine(int type, const void* Y, size_t rows, si
     return with_pieces(type, rows_vector(type, Y, ldy) && rows_vector(type, out, ldo), width, [&](auto t, auto n) {
         return with_grid(a, n(), [&](unsigned grid, bool many) {
             auto kernel = many ? route_combine_kernel<decltype(t), n(), 4, 1> : route_combine_kernel<decltype(t), n(), 1, 8>;
-            kernel<<<grid, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
+            return launch_kernel(kernel, grid, R_THREADS, static_cast<cudaStream_t>(cuda_stream), a);
         });
     });
 }
@@ -623,7 +622,6 @@ extern "C" int b200_sgemm_route_combine_backward(int type, const void* d_out, si
     a.rows     = (int)rows;
     const bool vector = rows_vector(type, d_out, ldo) && (!d_weights || rows_vector(type, Y, ldy)) && (!dY || rows_vector(type, dY, lddy));
     return with_pieces(type, vector, width, [&](auto t, auto n) {
-        route_backward_kernel<decltype(t), n()><<<(unsigned)tokens, R_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
-        return (int)cudaPeekAtLastError();
+        return launch_kernel(route_backward_kernel<decltype(t), n()>, (unsigned)tokens, R_THREADS, static_cast<cudaStream_t>(cuda_stream), a);
     });
 }
