@@ -202,7 +202,10 @@ namespace
             }
             cudaError_t e = cudaMalloc(&a.ptr, bytes);
             if(e != cudaSuccess)
+            {
+                (void)cudaGetLastError(); // the caller is told: keep it out of later launches' checks
                 return e;
+            }
             e = cudaMemsetAsync(a.ptr, 0, ARENA_FLAG_BYTES, stream);
             if(e != cudaSuccess)
             {

@@ -70,7 +70,10 @@ cudaError_t scratch_get(cudaStream_t stream, size_t bytes, void** out)
             s.bytes = 0;
         }
         if((e = cudaMalloc(&s.ptr, bytes)) != cudaSuccess)
+        {
+            (void)cudaGetLastError(); // the caller is told: keep it out of later launches' checks
             return e;
+        }
         s.bytes = bytes;
     }
     *out = s.ptr;

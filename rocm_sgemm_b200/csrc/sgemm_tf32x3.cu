@@ -495,6 +495,8 @@ cudaError_t grow(float** p, size_t* have, size_t need, cudaStream_t stream)
     cudaError_t e = cudaMalloc(p, need);
     if(e == cudaSuccess)
         *have = need;
+    else
+        (void)cudaGetLastError(); // the caller is told: keep it out of later launches' checks
     return e;
 }
 

@@ -29,3 +29,17 @@ def test_a_failed_allocation_does_not_fail_later_calls(sgemm):
     assert torch.equal(out, a)
     sgemm.route_combine_backward(f32, a, a, 64, 64, slot_row, 64, 1, weights, out, weights)
     assert torch.equal(out, a)
+
+
+@gpu
+def test_a_failed_allocation_does_not_fail_later_fp32_products(sgemm):
+    """The same refusal, then products whose launches are checked by the thread's last error."""
+    a, b, c = (torch.randn(96, 96, device="cuda") for _ in range(3))
+    assert sgemm.lib().b200_sgemm_3xtf32(1, 1, 1, a.data_ptr(), a.data_ptr(), a.data_ptr(), 1 << 20, 64, 1 << 18, None) > 0
+    want = (a.double() @ b.double()).float()
+    at = a.T.contiguous()  # col-major A, row-major B: both are copied
+    sgemm.gemm_3xtf32(0, 1, 0, c, at, b, 96, 96, 96)
+    assert torch.allclose(c, want, atol=1e-3)
+    c.zero_()
+    sgemm.gemm(0, 0, 0, c, a, b, 96, 96, 96)
+    assert torch.allclose(c, want, atol=1e-3)
