@@ -356,7 +356,7 @@ int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const void* a_codes,
                            const int* counts, size_t used_rows, float alpha, const float* global_a, const float* global_b,
                            void* cuda_stream);
 
-/* How a product is cut on a device with sm_count SMs, without touching one: *columns of a tile (64, 128, or 256 by pairs of
+/* How a product is cut on a device with sm_count (>= 2) SMs, without touching one: *columns of a tile (64, 128, or 256 by pairs of
  * CTAs; 0: the kernel for one or two rows) and the CTAs that share a tile's K (*split).  groups = 0: b200_sgemm_mx4; otherwise
  * b200_sgemm_mx4_grouped with M = used_rows (rows, where that is smaller or used_rows is 0) and a row-major C. */
 int b200_sgemm_mx4_plan(int layout_c, int type_c, size_t M, size_t N, size_t K, size_t groups, int sm_count, int* columns, int* split);

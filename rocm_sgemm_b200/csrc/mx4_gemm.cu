@@ -1204,7 +1204,7 @@ extern "C" int b200_sgemm_mx4_grouped(int format, int type_c, void* C, const voi
 extern "C" int b200_sgemm_mx4_plan(int layout_c, int type_c, size_t M, size_t N, size_t K, size_t groups, int sm_count, int* columns,
                                    int* split)
 {
-    if(!columns || !split || M == 0 || N == 0 || K == 0 || !type_ok(type_c) || layout_c & ~1 || sm_count < 1
+    if(!columns || !split || M == 0 || N == 0 || K == 0 || !type_ok(type_c) || layout_c & ~1 || sm_count < 2
        || (groups && layout_c != B200_SGEMM_ROW_MAJOR))
         return B200_SGEMM_INVALID_ARGUMENT;
     if(M > MAX_EXTENT || N > MAX_EXTENT || K > MAX_EXTENT || groups > G_MAX_GROUPS || groups * N > MAX_EXTENT)

@@ -51,6 +51,7 @@ def test_plan_refuses(sgemm):
     for kw in (dict(M=1 << 31), dict(N=1 << 31), dict(K=1 << 31), dict(groups=1025), dict(groups=1024, N=1 << 22)):
         assert call(**kw) == pkg.UNSUPPORTED_SIZE, kw
     assert sgemm.lib().b200_sgemm_mx4_plan(0, 0, 4, 8, 32, 0, 148, None, None) == pkg.INVALID_ARGUMENT
+    assert call(sms=1) == pkg.INVALID_ARGUMENT and call(sms=2) == pkg.OK  # a pair of CTAs needs two
     assert plan(0, "f32", 1, 4096, 4096) == (0, 1)
 
 
