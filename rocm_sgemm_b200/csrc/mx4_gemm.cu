@@ -13,11 +13,11 @@
 // 128 of the lanes, half of Q's rows and all of Q's scales, and the first one issues for both.  A pair reads half of Q from the
 // L2 and from shared memory and issues half the scale copies per product.
 //
-// One persistent CTA per SM, 10 warps:
+// One persistent CTA per SM, 10 warps (12 where 128 sums a thread stay in registers: 10 and 11 only give theirs up):
 //   warps 0-7  accumulate and store.  The tensor core adds into its FP32 accumulator with truncation, so for an FP32
 //              result the accumulator is emptied into registers every 1024 or 2048 k and the parts are added there,
-//              rounded to nearest (relative error of the whole result with operands of a wide range, K = 16384: 1.2e-7 in parts
-//              of 256 k, 2.9e-7 of 1024, 5.3e-7 of 2048; an FP32 product on the FMA pipe 2.4e-7).  A bias of at most 2^-23 a
+//              rounded to nearest (relative error of the whole result with scales over 2^+-8, K = 4096 and 16384 alike: 1.6e-7 in
+//              parts of 512 k, 2.8e-7 of 1024, 5.3e-7 of 2048; an FP32 product on the FMA pipe 5.0e-7 and 1.0e-6).  A bias of at most 2^-23 a
 //              product of 64 k: it stays below a quarter of the smallest rounding of an FP16 result (2^-12) up to 2^15 k and of
 //              a BF16 one (2^-9) up to 2^18, so those keep one accumulator that long and empty it as FP32 results do beyond.
 //   warp 8     fetches the stages by TMA: the two operands' codes (256 k = rows of 128 bytes, 128-byte swizzle) and the scale
@@ -54,7 +54,9 @@ constexpr int G_SCALE_COL  = 256; // tensor-memory columns 0..255: accumulators;
 constexpr int G_MAX_GROUPS = 1024;
 constexpr int MAX_SPLIT    = 8; // CTAs that share a tile's K
 constexpr int CHUNK_F32    = 4; // K blocks (1024 k, 16 products) added inside the tensor core for an FP32 result
-constexpr int CHUNK_F32_WIDE = 8; // the same for 256 columns, whose one accumulator stands still while it is emptied
+// the same for 256 columns, whose one accumulator stands still while it is emptied: 4096 cube 38.7 us, 8192 cube 236, 8192 tokens'
+// experts 162; with 1024 k 44.9, 262 and 190
+constexpr int CHUNK_F32_WIDE = 8;
 constexpr int CHUNK_F16    = 1 << 7, CHUNK_BF16 = 1 << 10; // 2^15 and 2^18 k
 // Registers of the kernel that keeps 128 sums a thread: 12 warps are launched with 168 each; warps 8 to 11 give theirs up
 // and warps 0 to 7 take them: 256 x 224 + 128 x 56 = 384 x 168, exactly the launch's allocation, so the increase is always granted.

@@ -236,7 +236,8 @@ __device__ __forceinline__ size_t scale_at(long long row, int block, int tiles)
 
 // K-contiguous source.  One CTA: 32 rows (a quarter of a band) x 512 k.  A warp takes four rows, the next fetched while one is
 // worked on, a lane 16 neighbours of each in one or two 32-byte loads; codes leave in contiguous pieces of a warp's width.  Scales meet in shared
-// memory and leave as words of four blocks.  (With a whole band per CTA, 16 rows per warp one after the other, 16384 x 8192
+// memory and leave as words of four blocks.  Rows off 32 bytes are read element by element: 16384 x 8192 BF16 70 us for nvfp4, 16384 x
+// 8200 140.  (With a whole band per CTA, 16 rows per warp one after the other, 16384 x 8192
 // BF16 took 163 us and 4097 x 2050 had only 165 CTAs.)
 template<int FMT, class T>
 __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_constant__ QArgs a)
@@ -328,8 +329,8 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_rows_kernel(const __grid_c
 
 // Row-contiguous source (a col-major A, a row-major B).  One CTA: a band of 128 rows x 128 k.  A thread takes one row (FP32) or
 // two neighbours (16 bits, one load of both), 32 k at a time; lanes take neighbouring rows, so a warp loads 128 contiguous
-// bytes of a k, and a thread has whole blocks in registers; three CTAs an SM.  (16384 x 8192 BF16: 106 us for nvfp4, 123 us with two
-// CTAs an SM, 68 us for mxfp4; with one row per thread of 16-bit types, 64 bytes a load, 270 us for
+// bytes of a k, and a thread has whole blocks in registers; three CTAs an SM.  (16384 x 8192 BF16: 93 us for nvfp4, with the matrix scale
+// amax / 2688 98, 68 us for mxfp4; with two CTAs an SM 123 us for nvfp4; with one row per thread of 16-bit types, 64 bytes a load, 270 us for
 // 16384 x 8192 BF16.)
 template<int FMT, class T>
 __global__ void __launch_bounds__(Q_THREADS, 3) quantize_cols_kernel(const __grid_constant__ QArgs a)

@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(R_THREADS) route_backward_kernel(const __grid_
     }
 }
 
-// f(type, pieces per vector) where all rows start on 16 bytes and hold whole pieces, else element by element
+// f(type, pieces per vector) where all rows start on 16 bytes and hold whole pieces, else element by element (8192 tokens x 4 BF16,
+// dispatch / combine / its gradients: width 2048 28.5 / 29.9 / 54.3 us, width 2050 36.9 / 56.3 / 90.7)
 template<class F>
 int with_pieces(int type, bool vector, size_t width, F f)
 {
