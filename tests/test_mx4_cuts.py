@@ -1,6 +1,7 @@
 """The ways in which the dispatcher cuts a 4-bit product (columns of a tile, CTAs that share its K): each is run."""
 import math
 import random
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -131,3 +132,31 @@ def test_grouped_of_every_tile(sgemm, fmt, columns, dtype):
             check(c[at], a[2][at], parts[e][2] * alpha, dtype)
         c[at] = 9
     assert (c == 9).all()
+
+
+@gpu
+def test_products_at_once(sgemm):
+    """Every kind of cut from threads of their own, on streams of their own, at the same time: the bits of calls made alone."""
+    shapes = [(1, 4096, 2048), (5, 5, 1796), (130, 397, 2369), (509, 517, 4094), (403, 131, 6150), (2100, 2300, 700), (1500, 700, 300)]
+    work = []
+    for i, (M, N, K) in enumerate(shapes):
+        fmt, dtype = FORMATS[i % 2], sorted(TYPES)[i % 3]
+        a, b = operand(fmt, M, K, 1), operand(fmt, N, K, 2)
+        c = [torch.zeros(M, N, dtype=TYPES[dtype], device="cuda") for _ in range(2)]
+        call = lambda out, stream, a=a, b=b, fmt=fmt, t=pkg.m_type[dtype], n=(M, N, K): sgemm.gemm_mx4(  # noqa: E731
+            fmt, 0, t, out, a[0], a[1], b[0], b[1], *n, alpha=2.0 ** -12, stream=stream)
+        call(c[0], torch.cuda.current_stream())
+        work.append((call, c, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def repeat(call, c, stream):
+        for _ in range(200):
+            call(c[1], stream)
+
+    with ThreadPoolExecutor(len(work)) as pool:
+        for done in [pool.submit(repeat, *w) for w in work]:
+            done.result()
+    torch.cuda.synchronize()
+    assert sgemm.mx4_device_status() == 0
+    for _, c, _ in work:
+        assert torch.isfinite(c[0]).all() and c[0].any() and torch.equal(*c)
